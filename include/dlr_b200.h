@@ -197,6 +197,135 @@ DLRB200_API int dlrb200_transpose_stack(const void* src, void* dst, int L, int r
 DLRB200_API int dlrb200_forward_static(const void* x, void* y, const void* Vp, const void* Up, int M, int d, int r,
                                        int L, float eps, int* status_dev, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The attention block of a locked decoder on a paged key-value cache.
+ *
+ * A cache holds pages of 2^n tokens (16 or more): k_cache and v_cache are (pages, kv_heads,
+ * page tokens, dim) tensors of 16-bit values with any strides (in elements,
+ * multiples of 8) and dim contiguous.  Slot s is token s % P of page s / P.  A
+ * request's row of the block table names its pages in the order of its tokens.
+ * There is no counterpart in the reference, whose decode loop leaves attention
+ * and cache to the host framework (dlr_lock/model.py:156-176 replaces only the
+ * MLP of a layer).  Like all calls of this library these are asynchronous on
+ * `stream`, allocate nothing and can be captured in a CUDA graph.
+ * ------------------------------------------------------------------------- */
+#define DLRB200_BF16 0
+#define DLRB200_F16 1
+#define DLRB200_MAX_PLAN_REQUESTS 8192
+
+/* One step's bookkeeping.  For request r, with len = 0 where finished[r] (its
+ * pages go back first): the tokens len .. len + new_tokens[r] - 1 get slots, the
+ * pages that are missing are taken from the top of the stack free_pages[0 ..
+ * n_free), in the order of the requests.  A request is refused, and keeps its
+ * length and pages, when it would pass columns pages, when its tokens do not fit
+ * its rows, or when it needs pages and those asked for up to and including it
+ * are more than there are.  Rows of the batch: `width` per request, or, with
+ * width 0, one request behind the other.  Rows without a token get slot -1 and
+ * position 0.  lengths_out and n_free_out may be lengths and n_free. */
+typedef struct dlrb200_plan_step {
+    const int* lengths;             /* (requests) tokens held */
+    const int* new_tokens;          /* (requests) */
+    const unsigned char* finished;  /* (requests) or null */
+    int* block_table;               /* (requests, columns), rows table_stride elements apart */
+    int64_t table_stride;
+    int* free_pages;                /* (pages) */
+    const int* n_free;              /* (1) */
+    int* slots;                     /* (rows) out */
+    int* positions;                 /* (rows) out */
+    int* starts;                    /* (requests + 1) out: each request's first row */
+    int* lengths_out;               /* (requests) */
+    int* n_free_out;                /* (1) */
+    int requests, columns, pages, page_size, width, rows;
+} dlrb200_plan_step;
+DLRB200_API int dlrb200_paged_plan(const dlrb200_plan_step* step, void* stream);
+
+/* RMS norm of every query and key head (left out where the weight is null),
+ * then the rotation by position of its first 2 * half values, rounded once:
+ *   n = x rsqrt(mean(x^2) + eps) w;  (a, b) -> (a cos - b sin, b cos + a sin)
+ * for the pairs (i, i + half), or (2 i, 2 i + 1) if interleaved.  With k_out the
+ * keys go there; without it keys and values go to `slots` of the cache (rows
+ * whose slot is outside it are left out; slots must differ).  A position outside
+ * the tables makes the row NaN.  q_out and k_out are (tokens, heads, dim)
+ * contiguous; the inputs may have any strides that are multiples of 4 elements.
+ * dim is a multiple of 8 up to 256, half a multiple of 4 up to dim / 2. */
+typedef struct dlrb200_norm_rope_args {
+    const void* q;                  /* (tokens, q_heads, dim) */
+    const void* k;                  /* (tokens, k_heads, dim) */
+    const void* v;                  /* the same as k; null with k_out */
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides */
+    const void* q_weight;           /* (dim) or null */
+    const void* k_weight;
+    const float* cos;               /* (table_rows, half) */
+    const float* sin;
+    const void* positions;          /* (tokens) int32, or int64 */
+    void* q_out;
+    void* k_out;
+    const int* slots;               /* (tokens) */
+    void* k_cache;
+    void* v_cache;
+    int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    int64_t tokens;
+    int q_heads, k_heads, dim, half, table_rows, pages, page_size;
+    int type;                       /* DLRB200_BF16 or DLRB200_F16 */
+    int weights_f32, positions_64, interleaved;
+    float eps;
+} dlrb200_norm_rope_args;
+DLRB200_API int dlrb200_qk_norm_rope(const dlrb200_norm_rope_args* args, void* stream);
+
+/* The gradient: from those of q_out and k_out to those of q and k (contiguous)
+ * and of the weights (in their type; null where there is no weight).  Sums are
+ * fp32 in a fixed order.  workspace: dlrb200_qk_norm_rope_backward_workspace_bytes,
+ * 16-byte aligned, needed only with a weight. */
+typedef struct dlrb200_norm_rope_grad_args {
+    const void* q;
+    const void* k;
+    const void* q_grad;
+    const void* k_grad;
+    int64_t q_token, q_head, k_token, k_head, qg_token, qg_head, kg_token, kg_head;
+    const void* q_weight;
+    const void* k_weight;
+    const float* cos;
+    const float* sin;
+    const void* positions;
+    void* dq;
+    void* dk;
+    void* dq_weight;
+    void* dk_weight;
+    void* workspace;
+    size_t workspace_bytes;
+    int64_t tokens;
+    int q_heads, k_heads, dim, half, table_rows;
+    int type, weights_f32, positions_64, interleaved;
+    float eps;
+} dlrb200_norm_rope_grad_args;
+DLRB200_API size_t dlrb200_qk_norm_rope_backward_workspace_bytes(int dim);
+DLRB200_API int dlrb200_qk_norm_rope_backward(const dlrb200_norm_rope_grad_args* args, void* stream);
+
+/* out[r, h] = softmax over j < lengths[r] of (scale q[r, h] . k_j) times v_j, with
+ * the keys and values of head h / (heads / kv_heads) of request r's pages; zeros
+ * where lengths[r] is 0.  Lengths are read on the device (held to 0 .. columns
+ * pages), so that a captured call follows them.  A table entry outside the cache
+ * is never followed: it counts as a page of zeros.  dim is 64, 96, 128 or 256,
+ * pages have at least 16 tokens.  workspace: 16-byte aligned, used only during
+ * the call; calls that overlap need one each. */
+typedef struct dlrb200_paged_attention_args {
+    const void* q;                  /* (requests, heads, dim), strides multiples of 2 elements */
+    int64_t q_request, q_head;
+    const void* k_cache;
+    const void* v_cache;
+    int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;
+    const int* block_table;         /* (requests, columns), rows table_stride elements apart */
+    int64_t table_stride;
+    const int* lengths;             /* (requests) */
+    void* out;                      /* (requests, heads, dim) contiguous, 16-byte aligned */
+    void* workspace;
+    size_t workspace_bytes;
+    int requests, heads, kv_heads, dim, columns, pages, page_size, type;
+    float scale;
+} dlrb200_paged_attention_args;
+DLRB200_API size_t dlrb200_paged_attention_workspace_bytes(int heads, int kv_heads, int dim);
+DLRB200_API int dlrb200_paged_attention(const dlrb200_paged_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,6 +2,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <shared_mutex>
@@ -12,6 +13,9 @@
 #include "decode_cluster.h"
 #include "decode_tl.h"
 #include "fold.h"
+#include "norm_rope.h"
+#include "paged_attention.h"
+#include "paged_plan.h"
 #include "resident.h"
 #include "stream.h"
 #include "stream_pair.h"
@@ -716,6 +720,162 @@ int dlrb200_forward_static(const void* x, void* y, const void* Vp, const void* U
     // the striped launcher clears the counter and the accumulator slots it uses on the
     // stream before the kernel, so whatever the previous call left behind does not matter
     return striped_forward(x, y, Vp, Up, M, d, r, L, eps, scratch, status_dev, static_cast<cudaStream_t>(stream), di);
+}
+
+// ---------------------------------------------------------------------------
+// The attention block on a paged cache.
+// ---------------------------------------------------------------------------
+namespace {
+
+// log2 of a page size, or -1
+int page_shift_of(int page_size) {
+    if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
+    int s = 0;
+    while ((1 << s) < page_size) ++s;
+    return s;
+}
+
+bool multiples(int64_t of, std::initializer_list<int64_t> values) {
+    for (int64_t v : values)
+        if (v % of) return false;
+    return true;
+}
+
+int device_b200(DevInfo* di) {
+    const int rc = device_info(di);
+    if (rc != DLRB200_OK) return rc;
+    return di->cc_major == 10 ? DLRB200_OK : DLRB200_ERR_CUDA;
+}
+
+int shape_of_heads(int q_heads, int k_heads, int dim, int half) {
+    if (q_heads <= 0 || k_heads <= 0 || dim <= 0 || half < 0) return DLRB200_ERR_INVALID_ARG;
+    return dim % 8 || dim > 256 || half % 4 || half > dim / 2 ? DLRB200_ERR_UNSUPPORTED_SHAPE : DLRB200_OK;
+}
+
+}  // namespace
+
+int dlrb200_paged_plan(const dlrb200_plan_step* s, void* stream) {
+    if (!s || s->requests < 0 || s->columns < 0 || s->pages < 0 || s->width < 0 || s->rows < 0) return DLRB200_ERR_INVALID_ARG;
+    const int shift = page_shift_of(s->page_size);
+    if (shift < 0 || s->requests > DLRB200_MAX_PLAN_REQUESTS || (int64_t(s->pages) << shift) > 0x7fffffff) return DLRB200_ERR_UNSUPPORTED_SHAPE;
+    if (s->width > 0 && int64_t(s->width) * s->requests != s->rows) return DLRB200_ERR_INVALID_ARG;
+    if (!s->n_free || !s->starts || !s->n_free_out || (s->rows > 0 && (!s->slots || !s->positions)) || (s->pages > 0 && !s->free_pages) ||
+        (s->requests > 0 && (!s->lengths || !s->new_tokens || !s->lengths_out || (s->columns > 0 && !s->block_table))))
+        return DLRB200_ERR_INVALID_ARG;
+    DevInfo di;
+    const int rc = device_b200(&di);
+    if (rc != DLRB200_OK) return rc;
+    dlr::PlanArgs a{};
+    a.lengths = s->lengths, a.new_tokens = s->new_tokens, a.finished = s->finished;
+    a.block_table = s->block_table, a.table_stride = s->table_stride, a.columns = s->columns;
+    a.free_pages = s->free_pages, a.pool = s->pages, a.n_free = s->n_free;
+    a.requests = s->requests, a.page_shift = shift, a.width = s->width, a.rows = s->rows;
+    a.slots = s->slots, a.positions = s->positions, a.starts = s->starts;
+    a.lengths_out = s->lengths_out, a.n_free_out = s->n_free_out;
+    return cuda_ok(dlr::paged_plan(a, di.smem_optin, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
+}
+
+int dlrb200_qk_norm_rope(const dlrb200_norm_rope_args* s, void* stream) {
+    if (!s || s->tokens < 0 || s->table_rows < 0 || (s->type != DLRB200_BF16 && s->type != DLRB200_F16)) return DLRB200_ERR_INVALID_ARG;
+    int rc = shape_of_heads(s->q_heads, s->k_heads, s->dim, s->half);
+    if (rc != DLRB200_OK) return rc;
+    const bool cache = s->k_out == nullptr;
+    const int shift = cache ? page_shift_of(s->page_size) : 0;
+    if (cache && (shift < 0 || s->pages < 0 || (int64_t(s->pages) << shift) > 0x7fffffff)) return DLRB200_ERR_UNSUPPORTED_SHAPE;
+    if (s->tokens == 0) return DLRB200_OK;
+    if (!s->q || !s->k || !s->q_out || !s->positions || (s->half > 0 && s->table_rows > 0 && (!s->cos || !s->sin))) return DLRB200_ERR_INVALID_ARG;
+    if (cache && (!s->v || !s->slots || (s->pages > 0 && (!s->k_cache || !s->v_cache)))) return DLRB200_ERR_INVALID_ARG;
+    if (!multiples(4, {s->q_token, s->q_head, s->k_token, s->k_head}) || !aligned(s->q, 8) || !aligned(s->k, 8) || !aligned(s->q_out, 8) ||
+        !aligned(s->k_out, 8) || !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16))
+        return DLRB200_ERR_ALIGNMENT;
+    if (cache && (!multiples(4, {s->v_token, s->v_head, s->kc_page, s->kc_head, s->kc_slot, s->vc_page, s->vc_head, s->vc_slot}) ||
+                  !aligned(s->v, 8) || !aligned(s->k_cache, 8) || !aligned(s->v_cache, 8)))
+        return DLRB200_ERR_ALIGNMENT;
+    DevInfo di;
+    rc = device_b200(&di);
+    if (rc != DLRB200_OK) return rc;
+    dlr::NormRope a{};
+    a.q = {s->q, s->q_token, s->q_head}, a.k = {s->k, s->k_token, s->k_head};
+    if (cache) a.v = {s->v, s->v_token, s->v_head};
+    a.q_weight = s->q_weight, a.k_weight = s->k_weight, a.cos = s->cos, a.sin = s->sin, a.positions = s->positions;
+    a.q_out = s->q_out, a.k_out = s->k_out, a.slots = s->slots, a.k_cache = s->k_cache, a.v_cache = s->v_cache;
+    a.k_page = s->kc_page, a.k_head = s->kc_head, a.k_slot = s->kc_slot;
+    a.v_page = s->vc_page, a.v_head = s->vc_head, a.v_slot = s->vc_slot;
+    a.n_slots = int64_t(s->pages) << shift, a.page_shift = shift;
+    a.tokens = s->tokens, a.q_heads = s->q_heads, a.k_heads = s->k_heads, a.dim = s->dim, a.half = s->half, a.table_rows = s->table_rows;
+    a.f16 = s->type == DLRB200_F16, a.weights_f32 = s->weights_f32 != 0, a.positions_64 = s->positions_64 != 0;
+    a.interleaved = s->interleaved != 0, a.eps = s->eps;
+    return cuda_ok(dlr::norm_rope(a, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
+}
+
+size_t dlrb200_qk_norm_rope_backward_workspace_bytes(int dim) {
+    DevInfo di;
+    if (dim <= 0 || dim > 256 || device_info(&di) != DLRB200_OK) return 0;
+    return size_t(dlr::norm_rope_partials(di.num_sms)) * dim * sizeof(float);
+}
+
+int dlrb200_qk_norm_rope_backward(const dlrb200_norm_rope_grad_args* s, void* stream) {
+    if (!s || s->tokens < 0 || s->table_rows < 0 || (s->type != DLRB200_BF16 && s->type != DLRB200_F16)) return DLRB200_ERR_INVALID_ARG;
+    int rc = shape_of_heads(s->q_heads, s->k_heads, s->dim, s->half);
+    if (rc != DLRB200_OK) return rc;
+    const bool weights = s->q_weight || s->k_weight;
+    if ((s->dq_weight && !s->q_weight) || (s->dk_weight && !s->k_weight)) return DLRB200_ERR_INVALID_ARG;
+    if (s->tokens > 0 && (!s->q_grad || !s->k_grad || !s->dq || !s->dk || !s->positions || (s->q_weight && !s->q) || (s->k_weight && !s->k) ||
+                          (s->half > 0 && s->table_rows > 0 && (!s->cos || !s->sin))))
+        return DLRB200_ERR_INVALID_ARG;
+    if (!multiples(4, {s->q_token, s->q_head, s->k_token, s->k_head, s->qg_token, s->qg_head, s->kg_token, s->kg_head}) || !aligned(s->q, 8) ||
+        !aligned(s->k, 8) || !aligned(s->q_grad, 8) || !aligned(s->k_grad, 8) || !aligned(s->dq, 8) || !aligned(s->dk, 8) ||
+        !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16))
+        return DLRB200_ERR_ALIGNMENT;
+    if (weights && (!s->workspace || s->workspace_bytes < dlrb200_qk_norm_rope_backward_workspace_bytes(s->dim))) return DLRB200_ERR_WORKSPACE;
+    if (weights && !aligned(s->workspace, 16)) return DLRB200_ERR_ALIGNMENT;
+    DevInfo di;
+    rc = device_b200(&di);
+    if (rc != DLRB200_OK) return rc;
+    dlr::NormRopeBackward a{};
+    a.q = {s->q, s->q_token, s->q_head}, a.k = {s->k, s->k_token, s->k_head};
+    a.q_grad = {s->q_grad, s->qg_token, s->qg_head}, a.k_grad = {s->k_grad, s->kg_token, s->kg_head};
+    a.q_weight = s->q_weight, a.k_weight = s->k_weight, a.cos = s->cos, a.sin = s->sin, a.positions = s->positions;
+    a.dq = s->dq, a.dk = s->dk, a.dq_weight = s->dq_weight, a.dk_weight = s->dk_weight, a.partial = static_cast<float*>(s->workspace);
+    a.tokens = s->tokens, a.q_heads = s->q_heads, a.k_heads = s->k_heads, a.dim = s->dim, a.half = s->half, a.table_rows = s->table_rows;
+    a.f16 = s->type == DLRB200_F16, a.weights_f32 = s->weights_f32 != 0, a.positions_64 = s->positions_64 != 0;
+    a.interleaved = s->interleaved != 0, a.eps = s->eps;
+    return cuda_ok(dlr::norm_rope_backward(a, di.num_sms, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
+}
+
+size_t dlrb200_paged_attention_workspace_bytes(int heads, int kv_heads, int dim) {
+    DevInfo di;
+    if (!dlr::paged_attention_supported(heads, kv_heads, dim) || device_info(&di) != DLRB200_OK) return 0;
+    return dlr::paged_attention_workspace_bytes(heads, kv_heads, dim, di.num_sms);
+}
+
+int dlrb200_paged_attention(const dlrb200_paged_attention_args* s, void* stream) {
+    if (!s || s->requests < 0 || s->columns < 0 || s->pages < 0 || (s->type != DLRB200_BF16 && s->type != DLRB200_F16)) return DLRB200_ERR_INVALID_ARG;
+    const int shift = page_shift_of(s->page_size);
+    if (shift < 0 || !dlr::paged_attention_supported(s->heads, s->kv_heads, s->dim) || int64_t(s->requests) * s->heads > 0x7fffffff ||
+        (int64_t(s->columns) << shift) > (1 << 30))
+        return DLRB200_ERR_UNSUPPORTED_SHAPE;
+    if (s->requests == 0) return DLRB200_OK;
+    // (an empty cache, or a table without columns, holds no tokens)
+    if (!s->q || !s->lengths || !s->out || (s->pages > 0 && (!s->k_cache || !s->v_cache)) || (s->columns > 0 && !s->block_table))
+        return DLRB200_ERR_INVALID_ARG;
+    if (!multiples(2, {s->q_request, s->q_head}) || !multiples(8, {s->kc_page, s->kc_head, s->kc_slot, s->vc_page, s->vc_head, s->vc_slot}) ||
+        !aligned(s->q, 4) || !aligned(s->k_cache, 16) || !aligned(s->v_cache, 16) || !aligned(s->out, 16) || !aligned(s->workspace, 16))
+        return DLRB200_ERR_ALIGNMENT;
+    if (!s->workspace || s->workspace_bytes < dlrb200_paged_attention_workspace_bytes(s->heads, s->kv_heads, s->dim)) return DLRB200_ERR_WORKSPACE;
+    DevInfo di;
+    const int rc = device_b200(&di);
+    if (rc != DLRB200_OK) return rc;
+    dlr::PagedAttention a{};
+    a.q = s->q, a.q_request = s->q_request, a.q_head = s->q_head;
+    a.k_cache = s->k_cache, a.v_cache = s->v_cache;
+    a.k_page = s->kc_page, a.k_head = s->kc_head, a.k_slot = s->kc_slot;
+    a.v_page = s->vc_page, a.v_head = s->vc_head, a.v_slot = s->vc_slot;
+    a.block_table = s->block_table, a.table_stride = s->table_stride, a.lengths = s->lengths, a.out = s->out, a.workspace = s->workspace;
+    a.requests = s->requests, a.heads = s->heads, a.kv_heads = s->kv_heads, a.dim = s->dim;
+    a.columns = s->pages > 0 ? s->columns : 0, a.page_shift = shift, a.pages = s->pages;
+    a.f16 = s->type == DLRB200_F16, a.scale = s->scale;
+    return cuda_ok(dlr::paged_attention(a, di.num_sms, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
 }
 
 }  // extern "C"

@@ -1,0 +1,524 @@
+// Attention of one new token per request over a paged key-value cache:
+//
+//   o_h = sum_j softmax_j(scale * q_h . k_j) v_j     over the tokens j of the request; zeros where there are none
+//
+// Bound by memory: the keys and values of a request are read once for all query heads that share them (64 bytes per
+// multiply-add of each of dim values and head: far below what the tensor cores give), and nothing else is big.
+//
+// Split.  The work is a list of tiles of 64 tokens: request by request, key-value head by key-value head.  It is cut into
+// equal runs, one per CTA, wherever the cuts fall: short requests share a CTA, a long one is spread over all of them, ragged
+// batches stay balanced, and the host needs to know no length.  A CTA works through its run segment by segment (the tiles of
+// one request and head).  What is cut is joined by a second, small kernel from partial results in fp32, in the order of the
+// tokens, so that results repeat bit for bit; what is whole is finished by its CTA.
+//
+// A warp takes 16 tokens of a tile at a time, on its own: it copies their keys and values to its own ring in shared memory
+// (cp.async, rows padded by 16 bytes so that ldmatrix meets no bank twice), multiplies with mma.sync, and keeps maximum, sum
+// and output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  The 16 rows of the
+// instruction hold up to 16 heads that share the keys; with up to eight, rows 8 to 15 of the second product hold what the
+// rounding of the softmax weights to 16 bits left over, so that weights count with twice the bits at no cost (with more, a
+// second instruction does that).
+#include "paged_attention.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace dlr {
+
+namespace {
+
+constexpr int kWarpsA = 4;
+constexpr int kThreadsA = 32 * kWarpsA;
+constexpr int kUnit = 16;                        // tokens of a warp's step
+constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
+constexpr int kMostCtasPerSm = 2;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D, int NT>
+struct Shape {
+    static constexpr int kRow = D * 2 + 16;                        // bytes of a row in shared memory
+    static constexpr int kHalf = kUnit * kRow;                     // keys (or values) of a step
+    static constexpr int kStage = 2 * kHalf;
+    static constexpr int kStages = D <= 128 ? 3 : 2;
+    static constexpr int kRing = kWarpsA * kStages * kStage;
+    static constexpr int kRows = 8 * NT;                           // query heads of a segment
+    static constexpr int kJoin = kWarpsA * kRows * (D + 4) * 4;    // output of every warp, and its maxima and sums behind
+    static constexpr int kJoinRow = D + 4;                         // floats; 16 bytes of padding
+    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kWarpsA * kRows * 8;
+    static constexpr int kCtasPerSm = kSmem <= 113 * 1024 ? 2 : 1;
+    static constexpr int kPart = kRows * (D + 2);                  // floats of a partial result: output, maxima, sums
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+                 : "r"(addr));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, __half)) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
+
+// two values rounded to 16 bits, and what that left over, rounded likewise
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if constexpr (__is_same(T, __half)) {
+        const __half2 h = __floats2half2_rn(x, y);
+        const float2 f = __half22float2(h);
+        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+        hi = *reinterpret_cast<const uint32_t*>(&h);
+        lo = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        hi = pack_bf16x2(x, y);
+        lo = pack_bf16x2(x - bf16lo_to_f(hi), y - bf16hi_to_f(hi));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    if constexpr (__is_same(T, __half)) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        return pack_bf16x2(x, y);
+    }
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(~0u, v, 1));
+    return fmaxf(v, __shfl_xor_sync(~0u, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(~0u, v, 1);
+    return v + __shfl_xor_sync(~0u, v, 2);
+}
+
+// Tokens and tiles of a request.
+struct Geometry {
+    const int* lengths;
+    int requests, segments;              // segments of a request: key-value heads x groups of query heads
+    long long capacity;
+
+    __device__ __forceinline__ int tokens(int r) const {
+        const long long n = lengths[r];
+        return int(n < 0 ? 0 : n > capacity ? capacity : n);
+    }
+    __device__ __forceinline__ long long tiles(int r) const { return (long long)((tokens(r) + kTile - 1) / kTile) * segments; }
+};
+
+// Sums of v over the warps' lanes: what lies before this thread, and all.
+template <int WARPS>
+__device__ __forceinline__ long long scan_tiles(long long v, long long* scratch, long long* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(~0u, sum, o);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += scratch[w];
+        all += scratch[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + sum - v;
+}
+
+// Tiles per CTA for `total` tiles.
+__device__ __forceinline__ long long run_of(long long total, int ctas) {
+    const long long even = (total + ctas - 1) / ctas;
+    return even < 1 ? 1 : even;
+}
+
+// The request that holds tile `at`, and the tiles before it.
+struct Place {
+    int request;
+    long long before;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid_constant__ PagedAttention p, int groups) {
+    using S = Shape<D, NT>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long scratch[kWarpsA];
+    __shared__ Place place;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int group_size = p.heads / p.kv_heads;
+    const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
+
+    // all tiles, then the request in which this CTA's run begins
+    long long total = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+        const int r = r0 + int(threadIdx.x);
+        long long here;
+        scan_tiles<kWarpsA>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
+        total += here;
+    }
+    const long long run = run_of(total, gridDim.x);
+    long long at = run * blockIdx.x;
+    const long long end = at + run < total ? at + run : total;
+    // requests without tokens belong to no tile: their zeros are written by the CTAs in turn
+    for (int r = blockIdx.x; r < p.requests; r += gridDim.x)
+        if (geo.tokens(r) == 0)
+            for (int i = threadIdx.x; i < p.heads * D / 2; i += kThreadsA)
+                reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + int64_t(r) * p.heads * D)[i] = 0;
+    if (at >= end) return;
+    long long base = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+        const int r = r0 + int(threadIdx.x);
+        const long long mine = r < p.requests ? geo.tiles(r) : 0;
+        long long here;
+        const long long before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
+        if (at >= before && at < before + mine) place = {r, before};
+        base += here;
+    }
+    __syncthreads();
+    int request = place.request;
+    long long before = place.before;
+
+    const uint32_t ring = smem_u32(smem) + warp * (S::kStages * S::kStage);
+    float* const join = reinterpret_cast<float*>(smem);
+    float2* const join_ml = reinterpret_cast<float2*>(smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin));
+    const float scale = p.scale * kLog2e;
+
+    for (; at < end;) {
+        // the segment that holds tile `at`
+        const int tokens = geo.tokens(request);
+        const int seg_tiles = (tokens + kTile - 1) / kTile;
+        if (at >= before + (long long)seg_tiles * geo.segments) {
+            before += (long long)seg_tiles * geo.segments;
+            ++request;
+            continue;
+        }
+        const int segment = int((at - before) / seg_tiles);
+        const int tile0 = int(at - before - (long long)segment * seg_tiles);
+        const long long left = end - at;
+        const int tile1 = seg_tiles - tile0 < left ? seg_tiles : tile0 + int(left);
+        const int kv_head = segment / groups, group = segment - kv_head * groups;
+        const int head0 = kv_head * group_size + group * S::kRows;
+        const int rows = min(S::kRows, group_size - group * S::kRows);
+        const int* const table = p.block_table + request * p.table_stride;
+        const T* const k_head = static_cast<const T*>(p.k_cache) + kv_head * p.k_head;
+        const T* const v_head = static_cast<const T*>(p.v_cache) + kv_head * p.v_head;
+
+        // this warp's steps: unit u covers the 16 tokens from u * 16, u = first, first + 4, ...
+        const int first = tile0 * kWarpsA + warp;
+        const int units = min(tile1 * kWarpsA, (tokens + kUnit - 1) / kUnit);
+        const int steps = first < units ? (units - first + kWarpsA - 1) / kWarpsA : 0;
+
+        // pages of the steps to come: lane i holds that of step 32 * n + i
+        int page_ids = 0;
+        auto load_pages = [&](int step) {
+            const int s = step + lane;
+            int id = -1;
+            if (s < steps) id = table[((first + s * kWarpsA) * kUnit) >> p.page_shift];
+            page_ids = id;
+        };
+        auto fetch = [&](int step) {
+            if (step < steps) {
+                if ((step & 31) == 0) load_pages(step);
+                const int page = __shfl_sync(~0u, page_ids, step & 31);
+                const int token0 = (first + step * kWarpsA) * kUnit;
+                const int slot0 = token0 & ((1 << p.page_shift) - 1);
+                const int valid = unsigned(page) < unsigned(p.pages) ? min(kUnit, tokens - token0) : 0;
+                const T* const k = k_head + (valid ? page : 0) * p.k_page;
+                const T* const v = v_head + (valid ? page : 0) * p.v_page;
+                const uint32_t stage = ring + (step % S::kStages) * S::kStage;
+                constexpr int kChunks = D / 8;
+#pragma unroll
+                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
+                    const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
+                    const uint32_t bytes = row < valid ? 16 : 0;
+                    const int slot = row < valid ? slot0 + row : 0;
+                    cp_async16(stage + row * S::kRow + col * 16, k + slot * p.k_slot + col * 8, bytes);
+                }
+#pragma unroll
+                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
+                    const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
+                    const uint32_t bytes = row < valid ? 16 : 0;
+                    const int slot = row < valid ? slot0 + row : 0;
+                    cp_async16(stage + S::kHalf + row * S::kRow + col * 16, v + slot * p.v_slot + col * 8, bytes);
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) fetch(s);
+
+        // queries: row lane / 4 (and + 8), as the first operand of the products with 16 values each
+        uint32_t q[D / 16][2 * NT];
+        {
+            const uint32_t* row[2];
+            bool on[2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int h = lane / 4 + 8 * n;
+                on[n] = h < rows;
+                row[n] = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + request * p.q_request + (head0 + (on[n] ? h : 0)) * p.q_head) + lane % 4;
+            }
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    q[k][n] = on[n] ? row[n][k * 8] : 0u;
+                    q[k][NT + n] = on[n] ? row[n][k * 8 + 4] : 0u;
+                }
+        }
+
+        float o[D / 8][4], m[NT], l[NT];
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n] = -INFINITY;
+            l[n] = 0.f;
+        }
+
+        for (int step = 0; step < steps; ++step) {
+            cp_async_wait<S::kStages - 2>();
+            __syncwarp();                       // the step's copies are there, and every lane is done with the step before
+            fetch(step + S::kStages - 1);
+            const uint32_t stage = ring + (step % S::kStages) * S::kStage;
+            // scores of 16 tokens: two products of 8 tokens each
+            float s[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+            const uint32_t k_at = stage + ((lane & 7) + ((lane >> 4) & 1) * 8) * S::kRow + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4(k_at + k * 32, b0, b1, b2, b3);
+                if constexpr (NT == 1) {
+                    mma16816<T>(s[0], q[k][0], 0u, q[k][1], 0u, b0, b1);
+                    mma16816<T>(s[1], q[k][0], 0u, q[k][1], 0u, b2, b3);
+                } else {
+                    mma16816<T>(s[0], q[k][0], q[k][1], q[k][2], q[k][3], b0, b1);
+                    mma16816<T>(s[1], q[k][0], q[k][1], q[k][2], q[k][3], b2, b3);
+                }
+            }
+            const int valid = tokens - (first + step * kWarpsA) * kUnit;
+            float alpha[NT];
+            uint32_t hi[2 * NT], lo[2 * NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float x[4] = {s[0][2 * n] * scale, s[0][2 * n + 1] * scale, s[1][2 * n] * scale, s[1][2 * n + 1] * scale};
+                if (valid < kUnit) {
+                    const int t = (lane % 4) * 2;
+                    if (t >= valid) x[0] = -INFINITY;
+                    if (t + 1 >= valid) x[1] = -INFINITY;
+                    if (t + 8 >= valid) x[2] = -INFINITY;
+                    if (t + 9 >= valid) x[3] = -INFINITY;
+                }
+                const float top = fmaxf(m[n], quad_max(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))));
+                const float ref = top == -INFINITY ? 0.f : top;       // (nothing but weights of zero so far)
+                alpha[n] = exp2f(m[n] - ref);
+                m[n] = top;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - ref);
+                l[n] = l[n] * alpha[n] + ((x[0] + x[1]) + (x[2] + x[3]));
+                split2<T>(x[0], x[1], hi[n], lo[n]);
+                split2<T>(x[2], x[3], hi[NT + n], lo[NT + n]);
+            }
+            bool same = alpha[0] == 1.f;
+            if constexpr (NT == 2) same = same && alpha[1] == 1.f;
+            if (!__all_sync(~0u, same)) {
+#pragma unroll
+                for (int n = 0; n < D / 8; ++n) {
+                    o[n][0] *= alpha[0];
+                    o[n][1] *= alpha[0];
+                    o[n][2] *= alpha[NT - 1];
+                    o[n][3] *= alpha[NT - 1];
+                }
+            }
+            const uint32_t v_at = stage + S::kHalf + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kRow + ((lane >> 4) & 1) * 16;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                uint32_t b0, b1, b2, b3;
+                ldmatrix_x4_trans(v_at + n * 32, b0, b1, b2, b3);
+                if constexpr (NT == 1) {
+                    mma16816<T>(o[2 * n], hi[0], lo[0], hi[1], lo[1], b0, b1);
+                    mma16816<T>(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b2, b3);
+                } else {
+                    mma16816<T>(o[2 * n], hi[0], hi[1], hi[2], hi[3], b0, b1);
+                    mma16816<T>(o[2 * n + 1], hi[0], hi[1], hi[2], hi[3], b2, b3);
+                    mma16816<T>(o[2 * n], lo[0], lo[1], lo[2], lo[3], b0, b1);
+                    mma16816<T>(o[2 * n + 1], lo[0], lo[1], lo[2], lo[3], b2, b3);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncthreads();                        // the rings are free
+
+        // the warps' results: maxima and sums, outputs (both halves of the weights added up)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float sum = quad_sum(l[n]);
+            const int row = lane / 4 + 8 * n;
+            if (lane % 4 == 0) join_ml[warp * S::kRows + row] = make_float2(m[n], sum);
+            float* const at_row = join + (warp * S::kRows + row) * S::kJoinRow + (lane % 4) * 2;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                float2 v;
+                if constexpr (NT == 1) v = make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+                else v = make_float2(o[c][2 * n], o[c][2 * n + 1]);
+                *reinterpret_cast<float2*>(at_row + c * 8) = v;
+            }
+        }
+        __syncthreads();
+        const bool whole = tile0 == 0 && tile1 == seg_tiles;
+        float* const part = static_cast<float*>(p.workspace) + (int64_t(blockIdx.x) * 2 + (at == run * blockIdx.x ? 0 : 1)) * S::kPart;
+        for (int i = threadIdx.x; i < rows * (D / 2); i += kThreadsA) {
+            const int row = i / (D / 2), c = (i % (D / 2)) * 2;
+            float2 ml[kWarpsA];
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarpsA; ++w) {
+                ml[w] = join_ml[w * S::kRows + row];
+                top = fmaxf(top, ml[w].x);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
+            float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarpsA; ++w) {
+                const float f = exp2f(ml[w].x - ref);
+                const float2 x = *reinterpret_cast<const float2*>(join + (w * S::kRows + row) * S::kJoinRow + c);
+                sum += f * ml[w].y;
+                v.x += f * x.x;
+                v.y += f * x.y;
+            }
+            if (whole) {
+                const float inv = 1.f / sum;
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head0 + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
+            } else {
+                *reinterpret_cast<float2*>(part + row * D + c) = v;
+                if (c == 0) *reinterpret_cast<float2*>(part + S::kRows * D + row * 2) = make_float2(top, sum);
+            }
+        }
+        __syncthreads();                        // the rings are written again
+        at += tile1 - tile0;
+    }
+}
+
+// One CTA per segment: joins the runs over which it was cut.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreadsA) join_kernel(const __grid_constant__ PagedAttention p, int groups, int ctas) {
+    using S = Shape<D, NT>;
+    __shared__ long long scratch[kWarpsA];
+    __shared__ long long before_us;
+    const int segments = p.kv_heads * groups;
+    const int request = blockIdx.x / segments, segment = blockIdx.x - request * segments;
+    const Geometry geo{p.lengths, p.requests, segments, (long long)p.columns << p.page_shift};
+    long long total = 0;
+    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+        const int r = r0 + int(threadIdx.x);
+        long long here;
+        const long long before = total + scan_tiles<kWarpsA>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
+        if (r == request) before_us = before;
+        total += here;
+    }
+    __syncthreads();
+    const int seg_tiles = (geo.tokens(request) + kTile - 1) / kTile;
+    if (seg_tiles == 0) return;
+    const long long run = run_of(total, ctas);
+    const long long begin = before_us + (long long)segment * seg_tiles, end = begin + seg_tiles;
+    const int cta0 = int(begin / run), cta1 = int((end - 1) / run);
+    if (cta0 == cta1) return;                   // not cut
+    const int group_size = p.heads / p.kv_heads, kv_head = segment / groups, group = segment - kv_head * groups;
+    const int head0 = kv_head * group_size + group * S::kRows, rows = min(S::kRows, group_size - group * S::kRows);
+    const float* const workspace = static_cast<const float*>(p.workspace);
+    // the segment opens its CTA's run unless it begins inside it
+    auto part_of = [&](int c) { return workspace + (int64_t(c) * 2 + (begin <= run * c ? 0 : 1)) * S::kPart; };
+    for (int i = threadIdx.x; i < rows * (D / 2); i += kThreadsA) {
+        const int row = i / (D / 2), c = (i % (D / 2)) * 2;
+        float top = -INFINITY, sum = 0.f;
+        float2 v = make_float2(0.f, 0.f);
+        for (int cta = cta0; cta <= cta1; ++cta) {
+            const float* const part = part_of(cta);
+            const float2 ml = *reinterpret_cast<const float2*>(part + S::kRows * D + row * 2);
+            const float2 x = *reinterpret_cast<const float2*>(part + row * D + c);
+            const float next = fmaxf(top, ml.x), ref = next == -INFINITY ? 0.f : next;
+            const float f = exp2f(top - ref), g = exp2f(ml.x - ref);
+            top = next;
+            sum = sum * f + ml.y * g;
+            v.x = v.x * f + x.x * g;
+            v.y = v.y * f + x.y * g;
+        }
+        const float inv = 1.f / sum;
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head0 + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
+    }
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
+    using S = Shape<D, NT>;
+    auto kern = paged_attention_kernel<T, D, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return e;
+    const int group_size = a.heads / a.kv_heads, groups = (group_size + S::kRows - 1) / S::kRows;
+    const int ctas = S::kCtasPerSm * num_sms;
+    kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups);
+    join_kernel<T, D, NT><<<unsigned(a.requests) * a.kv_heads * groups, kThreadsA, 0, stream>>>(a, groups, ctas);
+    return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_d(const PagedAttention& a, int num_sms, cudaStream_t stream) {
+    return a.heads / a.kv_heads <= 8 ? launch<T, D, 1>(a, num_sms, stream) : launch<T, D, 2>(a, num_sms, stream);
+}
+
+template <typename T>
+cudaError_t launch_t(const PagedAttention& a, int num_sms, cudaStream_t stream) {
+    switch (a.dim) {
+        case 64: return launch_d<T, 64>(a, num_sms, stream);
+        case 96: return launch_d<T, 96>(a, num_sms, stream);
+        case 128: return launch_d<T, 128>(a, num_sms, stream);
+        case 256: return launch_d<T, 256>(a, num_sms, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+bool paged_attention_supported(int heads, int kv_heads, int dim) {
+    return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && (dim == 64 || dim == 96 || dim == 128 || dim == 256);
+}
+
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int dim, int num_sms) {
+    const int rows = heads / kv_heads <= 8 ? 8 : 16;
+    return size_t(kMostCtasPerSm) * num_sms * 2 * rows * (dim + 2) * sizeof(float);
+}
+
+cudaError_t paged_attention(const PagedAttention& a, int num_sms, cudaStream_t stream) {
+    return a.f16 ? launch_t<__half>(a, num_sms, stream) : launch_t<__nv_bfloat16>(a, num_sms, stream);
+}
+
+}  // namespace dlr

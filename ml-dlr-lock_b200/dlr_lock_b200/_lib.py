@@ -26,6 +26,31 @@ class Plan(ctypes.Structure):
     ]
 
 
+def _struct(name, **groups):
+    """A ctypes mirror of a struct of the header: field names by type, in the order of the header."""
+    kinds = {"p": ctypes.c_void_p, "l": ctypes.c_int64, "i": ctypes.c_int, "f": ctypes.c_float, "z": ctypes.c_size_t}
+    fields = [(f, kinds[kind[0]]) for kind, names in groups.items() for f in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields, "__doc__": f"Mirror of ``{name}``."})
+
+
+PlanStep = _struct(
+    "dlrb200_plan_step", p1="lengths new_tokens finished block_table", l1="table_stride",
+    p2="free_pages n_free slots positions starts lengths_out n_free_out", i1="requests columns pages page_size width rows")
+NormRopeArgs = _struct(
+    "dlrb200_norm_rope_args", p1="q k v", l1="q_token q_head k_token k_head v_token v_head",
+    p2="q_weight k_weight cos sin positions q_out k_out slots k_cache v_cache",
+    l2="kc_page kc_head kc_slot vc_page vc_head vc_slot tokens", i1="q_heads k_heads dim half table_rows pages page_size type",
+    i2="weights_f32 positions_64 interleaved", f1="eps")
+NormRopeGradArgs = _struct(
+    "dlrb200_norm_rope_grad_args", p1="q k q_grad k_grad", l1="q_token q_head k_token k_head qg_token qg_head kg_token kg_head",
+    p2="q_weight k_weight cos sin positions dq dk dq_weight dk_weight workspace", z1="workspace_bytes", l2="tokens",
+    i1="q_heads k_heads dim half table_rows type weights_f32 positions_64 interleaved", f1="eps")
+PagedAttentionArgs = _struct(
+    "dlrb200_paged_attention_args", p1="q", l1="q_request q_head", p2="k_cache v_cache",
+    l2="kc_page kc_head kc_slot vc_page vc_head vc_slot", p3="block_table", l3="table_stride", p4="lengths out workspace",
+    z1="workspace_bytes", i1="requests heads kv_heads dim columns pages page_size type", f1="scale")
+
+
 # name -> (restype, argtypes); one entry per declaration in include/dlr_b200.h
 _vp, _i, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 SIGNATURES = {
@@ -43,6 +68,12 @@ SIGNATURES = {
     "dlrb200_status_to_host": (_i, [_vp, _vp, _vp]),
     "dlrb200_set_status_mirror": (_i, [_vp, _vp]),
     "dlrb200_forward_static": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _vp, _vp]),
+    "dlrb200_paged_plan": (_i, [ctypes.POINTER(PlanStep), _vp]),
+    "dlrb200_qk_norm_rope": (_i, [ctypes.POINTER(NormRopeArgs), _vp]),
+    "dlrb200_qk_norm_rope_backward_workspace_bytes": (_sz, [_i]),
+    "dlrb200_qk_norm_rope_backward": (_i, [ctypes.POINTER(NormRopeGradArgs), _vp]),
+    "dlrb200_paged_attention_workspace_bytes": (_sz, [_i, _i, _i]),
+    "dlrb200_paged_attention": (_i, [ctypes.POINTER(PagedAttentionArgs), _vp]),
 }
 
 _lib = None
