@@ -242,16 +242,16 @@ DLRB200_API int dlrb200_paged_plan(const dlrb200_plan_step* step, void* stream);
 /* RMS norm of every query and key head (left out where the weight is null),
  * then the rotation by position of its first 2 * half values, rounded once:
  *   n = x rsqrt(mean(x^2) + eps) w;  (a, b) -> (a cos - b sin, b cos + a sin)
- * for the pairs (i, i + half), or (2 i, 2 i + 1) if interleaved.  With k_out the
- * keys go there; without it keys and values go to `slots` of the cache (rows
- * whose slot is outside it are left out; slots must differ).  A position outside
+ * for the pairs (i, i + half), or (2 i, 2 i + 1) if interleaved.  The keys go to
+ * k_out, or, with slots, keys and values to those slots of the cache (rows whose
+ * slot is outside it are left out; slots must differ), or the keys to both.  A position outside
  * the tables makes the row NaN.  q_out and k_out are (tokens, heads, dim)
  * contiguous; the inputs may have any strides that are multiples of 4 elements.
  * dim is a multiple of 8 up to 256, half a multiple of 4 up to dim / 2. */
 typedef struct dlrb200_norm_rope_args {
     const void* q;                  /* (tokens, q_heads, dim) */
     const void* k;                  /* (tokens, k_heads, dim) */
-    const void* v;                  /* the same as k; null with k_out */
+    const void* v;                  /* the same as k; null without slots */
     int64_t q_token, q_head, k_token, k_head, v_token, v_head; /* strides */
     const void* q_weight;           /* (dim) or null */
     const void* k_weight;
@@ -260,7 +260,7 @@ typedef struct dlrb200_norm_rope_args {
     const void* positions;          /* (tokens) int32, or int64 */
     void* q_out;
     void* k_out;
-    const int* slots;               /* (tokens) */
+    const int* slots;               /* (tokens) or null */
     void* k_cache;
     void* v_cache;
     int64_t kc_page, kc_head, kc_slot, vc_page, vc_head, vc_slot;

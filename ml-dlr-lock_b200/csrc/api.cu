@@ -779,12 +779,13 @@ int dlrb200_qk_norm_rope(const dlrb200_norm_rope_args* s, void* stream) {
     if (!s || s->tokens < 0 || s->table_rows < 0 || (s->type != DLRB200_BF16 && s->type != DLRB200_F16)) return DLRB200_ERR_INVALID_ARG;
     int rc = shape_of_heads(s->q_heads, s->k_heads, s->dim, s->half);
     if (rc != DLRB200_OK) return rc;
-    const bool cache = s->k_out == nullptr;
+    const bool cache = s->slots != nullptr;
     const int shift = cache ? page_shift_of(s->page_size) : 0;
     if (cache && (shift < 0 || s->pages < 0 || (int64_t(s->pages) << shift) > 0x7fffffff)) return DLRB200_ERR_UNSUPPORTED_SHAPE;
     if (s->tokens == 0) return DLRB200_OK;
     if (!s->q || !s->k || !s->q_out || !s->positions || (s->half > 0 && s->table_rows > 0 && (!s->cos || !s->sin))) return DLRB200_ERR_INVALID_ARG;
-    if (cache && (!s->v || !s->slots || (s->pages > 0 && (!s->k_cache || !s->v_cache)))) return DLRB200_ERR_INVALID_ARG;
+    if (!cache && !s->k_out) return DLRB200_ERR_INVALID_ARG;
+    if (cache && (!s->v || (s->pages > 0 && (!s->k_cache || !s->v_cache)))) return DLRB200_ERR_INVALID_ARG;
     if (!multiples(4, {s->q_token, s->q_head, s->k_token, s->k_head}) || !aligned(s->q, 8) || !aligned(s->k, 8) || !aligned(s->q_out, 8) ||
         !aligned(s->k_out, 8) || !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16))
         return DLRB200_ERR_ALIGNMENT;

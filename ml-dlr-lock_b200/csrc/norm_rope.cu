@@ -158,19 +158,31 @@ __global__ void __launch_bounds__(kThreadsN) norm_rope_kernel(const __grid_const
     const int heads = kind == 0 ? p.q_heads : p.k_heads;
     const int first = group * (U * kSide) + sub;
 
-    T* out;
-    int64_t out_head = p.dim;
-    if (kind == 0) {
-        out = static_cast<T*>(p.q_out) + token * p.q_heads * p.dim;
-    } else if (p.k_out) {
-        out = static_cast<T*>(p.k_out) + token * p.k_heads * p.dim;
-    } else {
+    // rows of heads that this warp writes: q_out or k_out, and the token's slot of the cache
+    T* const out = kind == 0 ? static_cast<T*>(p.q_out) + token * p.q_heads * p.dim
+                   : kind == 1 && p.k_out ? static_cast<T*>(p.k_out) + token * p.k_heads * p.dim : nullptr;
+    T* cached = nullptr;
+    int64_t cached_head = 0;
+    if (kind != 0 && p.slots) {
         const int64_t slot = p.slots[token];
-        if (slot < 0 || slot >= p.n_slots) return;       // a row without a place in the cache
-        const int64_t page = slot >> p.page_shift, at = slot & ((1 << p.page_shift) - 1);
-        out = kind == 1 ? static_cast<T*>(p.k_cache) + page * p.k_page + at * p.k_slot : static_cast<T*>(p.v_cache) + page * p.v_page + at * p.v_slot;
-        out_head = kind == 1 ? p.k_head : p.v_head;
+        if (slot >= 0 && slot < p.n_slots) {             // (a row without a place in the cache otherwise)
+            const int64_t page = slot >> p.page_shift, at = slot & ((1 << p.page_shift) - 1);
+            cached = kind == 1 ? static_cast<T*>(p.k_cache) + page * p.k_page + at * p.k_slot
+                               : static_cast<T*>(p.v_cache) + page * p.v_page + at * p.v_slot;
+            cached_head = kind == 1 ? p.k_head : p.v_head;
+        }
     }
+    if (!out && !cached) return;
+    auto store = [&](int h, const Runs& run, uint2 a, uint2 b) {
+        if (out) {
+            *reinterpret_cast<uint2*>(out + h * p.dim + run.a) = a;
+            *reinterpret_cast<uint2*>(out + h * p.dim + run.b) = b;
+        }
+        if (cached) {
+            *reinterpret_cast<uint2*>(cached + h * cached_head + run.a) = a;
+            *reinterpret_cast<uint2*>(cached + h * cached_head + run.b) = b;
+        }
+    };
 
     const Runs run = runs_of<INTERLEAVED>(l, p.half);
     const bool lane_on = 8 * l < p.dim;
@@ -189,10 +201,7 @@ __global__ void __launch_bounds__(kThreadsN) norm_rope_kernel(const __grid_const
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int h = first + u * kSide;
-            if (lane_on && h < heads) {
-                *reinterpret_cast<uint2*>(out + h * out_head + run.a) = va[u];
-                *reinterpret_cast<uint2*>(out + h * out_head + run.b) = vb[u];
-            }
+            if (lane_on && h < heads) store(h, run, va[u], vb[u]);
         }
         return;
     }
@@ -225,10 +234,7 @@ __global__ void __launch_bounds__(kThreadsN) norm_rope_kernel(const __grid_const
 #pragma unroll
             for (int i = 0; i < 4; ++i) a[i] = b[i] = __int_as_float(0x7fffffff);
         const int h = first + u * kSide;
-        if (lane_on && h < heads) {
-            *reinterpret_cast<uint2*>(out + h * out_head + run.a) = pack<T>(a);
-            *reinterpret_cast<uint2*>(out + h * out_head + run.b) = pack<T>(b);
-        }
+        if (lane_on && h < heads) store(h, run, pack<T>(a), pack<T>(b));
     }
 }
 

@@ -20,8 +20,8 @@ struct NormRope {
     const float* sin;
     const void* positions;               // (tokens)
     void* q_out;                         // (tokens, q_heads, dim) contiguous
-    void* k_out;                         // the same, or null where k and v go to the cache
-    const int* slots;                    // (tokens), cache only
+    void* k_out;                         // the same, or null
+    const int* slots;                    // (tokens): k and v go to the cache (k to k_out too, if there is one); or null
     void* k_cache;                       // (pages, k_heads, page tokens, dim), strides in elements
     void* v_cache;
     int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;

@@ -21,9 +21,10 @@ from .model import (  # noqa: F401
     set_fast_path,
     write_config,
 )
-from . import attention, evaluate, harness, ops, packed, registry, sharding  # noqa: F401
+from . import attention, evaluate, harness, ops, packed, registry, serving, sharding  # noqa: F401
 from .attention import PagedPlan, paged_attention, paged_plan, qk_norm_rope, qk_norm_rope_append, rope_tables  # noqa: F401
 from .evaluate import evaluate_ppl, synthetic_token_stream  # noqa: F401
 from .packed import PackedNet, load_packed_weights, pack_state_dict  # noqa: F401
+from .serving import PagedCache, PagedDecoder  # noqa: F401
 
 __version__ = "0.1.0"

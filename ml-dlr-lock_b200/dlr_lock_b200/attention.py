@@ -297,8 +297,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
                         k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                         slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *, eps: float = EPS,
-                        interleaved: bool = False) -> torch.Tensor:
-    """``qk_norm_rope`` for serving: returns the queries; keys, and ``v`` as it is, go to ``slots`` (...) int32 of the caches.
+                        interleaved: bool = False, return_keys: bool = False):
+    """``qk_norm_rope`` for serving: keys, and ``v`` as it is, go to ``slots`` (...) int32 of the caches; returns the queries,
+    and with ``return_keys`` the keys too (what the attention over a whole prompt takes).
 
     Rows whose slot is outside the caches (-1) are not stored; the others must name different slots.  No gradient.
     """
@@ -315,12 +316,13 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     device = _on_one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache)
     with torch.cuda.device(device):
         q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=device) if return_keys else None
         at, to = positions.reshape(-1).contiguous(), slots.reshape(-1).contiguous()
         if at.numel():
-            args = _forward_args(_flat(q), _flat(k), _vector(q_weight), _vector(k_weight), cos, sin, at, q_out, None, float(eps),
+            args = _forward_args(_flat(q), _flat(k), _vector(q_weight), _vector(k_weight), cos, sin, at, q_out, k_out, float(eps),
                                  interleaved, _flat(v), to, k_cache, v_cache)
             _lib.check(_lib.load().dlrb200_qk_norm_rope(ctypes.byref(args), _stream_ptr(device.index)), "dlrb200_qk_norm_rope")
-    return q_out
+    return (q_out, k_out) if return_keys else q_out
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------------

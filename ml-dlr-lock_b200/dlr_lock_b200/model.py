@@ -22,7 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.utils.checkpoint import checkpoint as _checkpoint
 
-from . import _lib, ops
+from . import _lib, attention, ops
 
 
 def dlrnet_param_count(d: int, r: int, depth: int) -> int:
@@ -309,19 +309,92 @@ def _fused_locked_layer_forward(self, hidden_states, **kwargs):
     return self.mlp.dlrnet(hidden_states + attn)
 
 
+class RotaryTables:
+    """Cosines and sines of a decoder's rotary embedding for every position up to its ``max_position_embeddings`` (or ``positions``),
+    fp32, made on first use on each device."""
+
+    def __init__(self, model, positions: Optional[int] = None):
+        self._rotary = model.model.rotary_emb
+        self._positions = int(positions if positions is not None else model.config.max_position_embeddings)
+        self._made = {}
+
+    @staticmethod
+    def fixed(model) -> bool:
+        """Whether the frequencies are the same at every length."""
+        rotary = getattr(model.model, "rotary_emb", None)
+        return rotary is not None and hasattr(rotary, "inv_freq") and getattr(rotary, "rope_type", "default") not in ("dynamic", "longrope")
+
+    def on(self, device):
+        device = torch.device(device)
+        if device not in self._made:
+            scale = float(getattr(self._rotary, "attention_scaling", 1.0))
+            self._made[device] = attention.rope_tables(self._rotary.inv_freq.detach().to(device), self._positions, scale)
+        return self._made[device]
+
+
+def head_norms(attn):
+    """(weight of the query norm, of the key norm, epsilon) of an attention module, None where it has no such norm."""
+    q, k = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+    if q is None and k is None:
+        return None, None, ops.EPS
+    return q.weight, k.weight, float(getattr(q, "variance_epsilon", ops.EPS))
+
+
+def attention_fusable(attn) -> bool:
+    """Whether an attention module is projections, norms over each head (or none) and a rotation, on full attention."""
+    if not all(hasattr(attn, n) for n in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "scaling", "layer_idx")):
+        return False
+    if getattr(attn, "sliding_window", None) or hasattr(attn, "sinks"):
+        return False
+    norms = [getattr(attn, n, None) for n in ("q_norm", "k_norm")]
+    if all(n is None for n in norms):
+        return True
+    return all(n is not None and getattr(n, "weight", None) is not None and n.weight.shape == (attn.head_dim,)
+               and getattr(n, "variance_epsilon", None) == getattr(norms[0], "variance_epsilon", None) for n in norms)
+
+
+def _fused_attention_forward(self, hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
+    """The host framework's attention with the norms of queries and keys and their rotation in one kernel
+    (``attention.qk_norm_rope``, with its gradient).  The attention function itself is the host framework's.  Takes the
+    module's own forward for anything but bf16 and fp16 on a GPU."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    positions, name = kwargs.get("position_ids"), self.config._attn_implementation
+    if not hidden_states.is_cuda or hidden_states.dtype not in (torch.bfloat16, torch.float16) or positions is None \
+            or name not in ALL_ATTENTION_FUNCTIONS or self.q_proj.weight.dtype != hidden_states.dtype:
+        return type(self).forward(self, hidden_states=hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
+                                  past_key_values=past_key_values, **kwargs)
+    rows = hidden_states.shape[:-1]
+    q, k, v = (proj(hidden_states).view(*rows, -1, self.head_dim) for proj in (self.q_proj, self.k_proj, self.v_proj))
+    q_weight, k_weight, eps = head_norms(self)
+    cos, sin = self._rotary_tables.on(hidden_states.device)
+    q, k = attention.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions.expand(rows), eps=eps)
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+    if past_key_values is not None:
+        at = kwargs.get("cache_position")
+        k, v = past_key_values.update(k, v, self.layer_idx, *(() if at is None else ({"cache_position": at},)))
+    out, weights = ALL_ATTENTION_FUNCTIONS[name](self, q, k, v, attention_mask, scaling=self.scaling,
+                                                 dropout=self.attention_dropout if self.training else 0.0, **kwargs)
+    return self.o_proj(out.reshape(*rows, -1).contiguous()), weights
+
+
 def _fusable(layer) -> bool:
     return (isinstance(getattr(layer, "mlp", None), ResidualDLRNet)
             and isinstance(getattr(layer, "post_attention_layernorm", None), nn.Identity)
             and hasattr(layer, "input_layernorm") and hasattr(layer, "self_attn"))
 
 
-def fuse_decoder_layers(model, enabled: bool = True) -> int:
+def fuse_decoder_layers(model, enabled: bool = True, attention: bool = False) -> int:
     """Switch every locked decoder layer of ``model`` between the host framework's own forward (the
     reference composition ``h + (dlrnet(h) - h)``) and the fused one (``dlrnet(h)``).  Only layers of the
     standard pre-norm form are touched (``input_layernorm``, ``self_attn``, an identity
-    ``post_attention_layernorm`` and a ``ResidualDLRNet`` as ``mlp``).  Returns how many were switched."""
+    ``post_attention_layernorm`` and a ``ResidualDLRNet`` as ``mlp``).  With ``attention`` their attention modules also take the
+    norms of queries and keys and the rotation as one kernel, forward and backward (modules of another form are left as
+    they are; the rotation is in fp32, the host framework's in the model's type, and covers ``max_position_embeddings``
+    positions).  Returns how many layers were switched."""
     import types
     n = 0
+    tables = RotaryTables(model) if enabled and attention and RotaryTables.fixed(model) else None
     for layer in model.model.layers:
         if not _fusable(layer):
             continue
@@ -329,6 +402,13 @@ def fuse_decoder_layers(model, enabled: bool = True) -> int:
             layer.forward = types.MethodType(_fused_locked_layer_forward, layer)
         elif "forward" in layer.__dict__:
             del layer.__dict__["forward"]
+        attn = layer.self_attn
+        if tables is not None and attention_fusable(attn):
+            attn._rotary_tables = tables
+            attn.forward = types.MethodType(_fused_attention_forward, attn)
+        elif "_rotary_tables" in attn.__dict__:
+            del attn.__dict__["_rotary_tables"]
+            del attn.__dict__["forward"]
         n += 1
     return n
 

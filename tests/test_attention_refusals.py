@@ -164,7 +164,7 @@ def test_the_c_abi_refuses_before_any_cuda_call(lib):
     norm = dict(q=at, k=at, q_token=64, q_head=64, k_token=64, k_head=64, cos=at, sin=at, positions=at, q_out=at, k_out=at, tokens=1,
                 q_heads=1, k_heads=1, dim=64, half=32, table_rows=1)
     for changed, code in ((dict(dim=60), 2), (dict(dim=264), 2), (dict(half=36), 2), (dict(half=30), 2), (dict(type=2), 1), (dict(q=None), 1),
-                          (dict(q_out=None), 1), (dict(k_out=None), 2), (dict(k_out=None, page_size=16), 1), (dict(q_head=63), 3),
+                          (dict(q_out=None), 1), (dict(k_out=None), 1), (dict(slots=at), 2), (dict(slots=at, page_size=16), 1), (dict(q_head=63), 3),
                           (dict(q=at + 2), 3), (dict(cos=at + 4), 3), (dict(tokens=-1), 1), (dict(tokens=0, q=None), 0)):
         assert lib.dlrb200_qk_norm_rope(ref(_lib.NormRopeArgs(**{**norm, **changed})), None) == code, changed
 

@@ -295,6 +295,9 @@ def test_append(tokens, heads, kv_heads, dim, half, dtype, order):
         changed = (cache.transpose(1, 2) != (old if order == "tokens first" else old.transpose(1, 2))).any(-1).any(-1).flatten()
         changed[slot] = False
         assert not changed.any()                             # everything else as it was
+    both = D.qk_norm_rope_append(q, k, v, qw, kw, cos, sin, positions, slots, *(c.clone() for c in (kc, vc)), eps=1e-5,
+                                 interleaved=interleaved, return_keys=True)
+    assert torch.equal(both[0], want_q) and torch.equal(both[1], want_k)
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------------
