@@ -242,4 +242,13 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&kModule); }
+extern PyMethodDef kAttentionMethods[];          // host_attention.cpp
+
+PyMODINIT_FUNC PyInit__host() {
+    PyObject* const m = PyModule_Create(&kModule);
+    if (m && PyModule_AddFunctions(m, kAttentionMethods) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

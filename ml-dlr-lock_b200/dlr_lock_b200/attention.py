@@ -16,15 +16,14 @@ graph; workspaces are taken from torch's allocator per call, so that captured gr
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .ops import EPS, _stream_ptr
+from .ops import EPS
 
-_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+_TYPES = (torch.bfloat16, torch.float16)
 MAX_REQUESTS = 8192                     # of one plan
 
 
@@ -35,6 +34,30 @@ class PagedPlan(NamedTuple):
     starts: torch.Tensor                # (requests + 1) first row of each request
     lengths: torch.Tensor               # (requests) tokens held after the step
     n_free: torch.Tensor                # (1) free pages after the step
+
+
+_bound = None
+
+
+def _native():
+    """The native side of these calls (csrc/host_attention.cpp), which takes arguments that are as the kernels read them and
+    returns None for all others."""
+    global _bound
+    if _bound is None:
+        lib, host = _lib.load(), _lib.host()
+        host.bind(*(ctypes.cast(getattr(lib, "dlrb200_" + name), ctypes.c_void_p).value
+                    for name in ("paged_plan", "qk_norm_rope", "qk_norm_rope_backward", "qk_norm_rope_backward_workspace_bytes",
+                                 "paged_attention", "paged_attention_workspace_bytes", "strerror")))
+        _bound = host
+    return _bound
+
+
+def _result(out, what):
+    if type(out) is int:
+        _lib.check(out, what)
+    if out is None:
+        raise RuntimeError(f"{what}: arguments that passed every check were not taken")
+    return out
 
 
 def _all_tensors(what, *tensors):
@@ -67,6 +90,8 @@ def _int32(what, name, t, shape):
 
 
 def _page_size(what, page_size):
+    if type(page_size) is not int:
+        raise TypeError(f"{what}: the page size must be an int, not {type(page_size).__name__}")
     if page_size < 16 or page_size & (page_size - 1):
         raise ValueError(f"{what}: pages have 2^n tokens, 16 or more, not {page_size}")
 
@@ -88,7 +113,8 @@ def _check_cache(what, k_cache, v_cache, dtype, kv_heads, dim, multiple):
 
 def _heads(t: torch.Tensor, multiple: int) -> torch.Tensor:
     """t if its rows can be read where they are, else a contiguous copy."""
-    if t.stride(-1) == 1 and not any(s % multiple for s in t.stride()[:-1]) and t.data_ptr() % (2 * multiple) == 0:
+    one = t.dim() <= 3 or t.is_contiguous()               # the leading dimensions are a single one
+    if one and t.stride(-1) == 1 and not any(s % multiple for s in t.stride()[:-1]) and t.data_ptr() % (2 * multiple) == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -109,6 +135,9 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
     when the table has no columns for its tokens, when they do not fit its rows, or when it needs pages and those asked for
     up to and including it are more than there are free.
     """
+    out = _native().paged_plan(lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
+    if type(out) is tuple:
+        return PagedPlan(*out)
     what = "paged_plan"
     _all_tensors(what, lengths, new_tokens, block_table, free_pages, n_free)
     if lengths.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
@@ -135,24 +164,15 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
         if width is None or rows != width * n:
             raise ValueError(f"{what}: give width, or width=None and rows")
     if width is not None:
-        if width < 1:
-            raise ValueError(f"{what}: width is at least 1")
+        if type(width) is not int or width < 1:
+            raise ValueError(f"{what}: width is an int, at least 1")
         rows = width * n
-    if rows < 0 or rows > 0x7fffffff:
+    if type(rows) is not int or rows < 0 or rows > 0x7fffffff:
         raise ValueError(f"{what}: {rows} rows")
     device = _on_one_device(what, lengths, new_tokens, block_table, free_pages, n_free, finished)
     with torch.cuda.device(device):
-        # one allocation: slots, positions, starts, lengths, count
-        out = torch.empty(2 * rows + 2 * n + 2, dtype=torch.int32, device=device)
-        slots, positions, starts, new_lengths, count = out.split([rows, rows, n + 1, n, 1])
-        if in_place:
-            new_lengths, count = lengths, n_free
-        step = _lib.PlanStep(lengths.data_ptr(), new_tokens.data_ptr(), finished.data_ptr() if finished is not None else None,
-                             block_table.data_ptr(), block_table.stride(0), free_pages.data_ptr(), n_free.data_ptr(),
-                             slots.data_ptr(), positions.data_ptr(), starts.data_ptr(), new_lengths.data_ptr(), count.data_ptr(),
-                             n, block_table.shape[1], free_pages.shape[0], page_size, width or 0, rows)
-        _lib.check(_lib.load().dlrb200_paged_plan(ctypes.byref(step), _stream_ptr(device.index)), "dlrb200_paged_plan")
-    return PagedPlan(slots, positions, starts, new_lengths, count)
+        out = _native().paged_plan(lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
+    return PagedPlan(*_result(out, "dlrb200_paged_plan"))
 
 
 # ---- norm and rotation ------------------------------------------------------------------------------------------------------
@@ -203,76 +223,9 @@ def _vector(w):
     return w.clone(memory_format=torch.contiguous_format)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _flat(t: torch.Tensor) -> torch.Tensor:
-    """(..., heads, dim) as (tokens, heads, dim), where it lies if that can be."""
-    return _heads(t.reshape(-1, *t.shape[-2:]) if t.dim() != 3 else t, 4)
-
-
-def _strides(t):
-    return t.stride(0), t.stride(1)
-
-
-def _forward_args(q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out, eps, interleaved, v=None, slots=None, k_cache=None, v_cache=None):
-    weight = q_weight if q_weight is not None else k_weight
-    kc, vc = ((*c.stride()[:3],) if c is not None else (0, 0, 0) for c in (k_cache, v_cache))
-    pages, page_size = (k_cache.shape[0], k_cache.shape[2]) if k_cache is not None else (0, 0)
-    return _lib.NormRopeArgs(
-        q.data_ptr(), k.data_ptr(), _ptr(v), *_strides(q), *_strides(k), *(_strides(v) if v is not None else (0, 0)),
-        _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), q_out.data_ptr(), _ptr(k_out),
-        _ptr(slots), _ptr(k_cache), _ptr(v_cache), *kc, *vc, q.shape[0], q.shape[1], k.shape[1], q.shape[2], cos.shape[1],
-        cos.shape[0], pages, page_size, _TYPES[q.dtype], int(weight is not None and weight.dtype == torch.float32),
-        int(positions.dtype == torch.int64), int(interleaved), eps)
-
-
-class _NormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        with torch.cuda.device(q.device):
-            q3, k3 = _flat(q), _flat(k)
-            qw, kw = _vector(q_weight), _vector(k_weight)
-            at = positions.reshape(-1).contiguous()
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            if at.numel():
-                args = _forward_args(q3, k3, qw, kw, cos, sin, at, q_out, k_out, eps, interleaved)
-                _lib.check(_lib.load().dlrb200_qk_norm_rope(ctypes.byref(args), _stream_ptr(q.get_device())), "dlrb200_qk_norm_rope")
-        # without a norm the gradient does not depend on the input
-        ctx.save_for_backward(q if q_weight is not None else None, k if k_weight is not None else None, q_weight, k_weight, cos, sin, positions)
-        ctx.eps, ctx.interleaved, ctx.shapes = eps, interleaved, (q.shape, k.shape)
-        return q_out, k_out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, q_grad, k_grad):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        device, dtype = q_grad.device, q_grad.dtype
-        with torch.cuda.device(device):
-            lib = _lib.load()
-            dq, dk = (torch.empty(s, dtype=dtype, device=device) for s in ctx.shapes)
-            dqw, dkw = (None if w is None else torch.empty(w.shape, dtype=w.dtype, device=device) for w in (q_weight, k_weight))
-            gq, gk = _flat(q_grad), _flat(k_grad)
-            q3, k3 = (None if t is None else _flat(t) for t in (q, k))
-            qw, kw = _vector(q_weight), _vector(k_weight)
-            at = positions.reshape(-1).contiguous()
-            weight = qw if qw is not None else kw
-            dim = gq.shape[2]
-            workspace, need = None, 0
-            if weight is not None:
-                need = lib.dlrb200_qk_norm_rope_backward_workspace_bytes(dim)
-                workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            none = (0, 0)
-            args = _lib.NormRopeGradArgs(
-                _ptr(q3), _ptr(k3), gq.data_ptr(), gk.data_ptr(), *(_strides(q3) if q3 is not None else none),
-                *(_strides(k3) if k3 is not None else none), *_strides(gq), *_strides(gk), _ptr(qw), _ptr(kw), cos.data_ptr(),
-                sin.data_ptr(), at.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw), _ptr(workspace), need,
-                gq.shape[0], gq.shape[1], gk.shape[1], dim, cos.shape[1], cos.shape[0], _TYPES[dtype],
-                int(weight is not None and weight.dtype == torch.float32), int(at.dtype == torch.int64), int(ctx.interleaved), ctx.eps)
-            _lib.check(lib.dlrb200_qk_norm_rope_backward(ctypes.byref(args), _stream_ptr(device.index)), "dlrb200_qk_norm_rope_backward")
-        return dq, dk, dqw, dkw, None, None, None, None, None
+def _in_shape(q, k, q_weight, k_weight, cos, sin, positions):
+    """The arguments laid out as the kernels read them; gradients pass through."""
+    return _heads(q, 4), _heads(k, 4), _vector(q_weight), _vector(k_weight), cos, sin, positions.contiguous()
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -286,12 +239,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     (2i, 2i + 1) with ``interleaved``; the rest passes through.  ``positions`` (...) int32 or int64; one outside the tables
     makes its row NaN.  fp32 throughout, rounded once.  Differentiable (once) in q, k and the weights.
     """
+    out = _native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if type(out) is tuple:
+        return out
     what = "qk_norm_rope"
     _check_norm_rope(what, q, k, q_weight, k_weight, cos, sin, positions)
     if cos.requires_grad or sin.requires_grad:
         raise ValueError(f"{what}: the tables have no gradient")
-    _on_one_device(what, q, k, q_weight, k_weight, cos, sin, positions)
-    return _NormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
+    device = _on_one_device(what, q, k, q_weight, k_weight, cos, sin, positions)
+    with torch.cuda.device(device):
+        out = _native().qk_norm_rope(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), float(eps), bool(interleaved))
+    return _result(out, "dlrb200_qk_norm_rope")
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
@@ -303,6 +261,10 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
 
     Rows whose slot is outside the caches (-1) are not stored; the others must name different slots.  No gradient.
     """
+    out = _native().qk_norm_rope_append(q, k, q_weight, k_weight, cos, sin, positions, v, slots, k_cache, v_cache, eps, interleaved,
+                                        return_keys)
+    if out is not None and type(out) is not int:
+        return out
     what = "qk_norm_rope_append"
     _all_tensors(what, v, slots, k_cache, v_cache)
     dim, _ = _check_norm_rope(what, q, k, q_weight, k_weight, cos, sin, positions)
@@ -315,14 +277,9 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
     device = _on_one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache)
     with torch.cuda.device(device):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=device) if return_keys else None
-        at, to = positions.reshape(-1).contiguous(), slots.reshape(-1).contiguous()
-        if at.numel():
-            args = _forward_args(_flat(q), _flat(k), _vector(q_weight), _vector(k_weight), cos, sin, at, q_out, k_out, float(eps),
-                                 interleaved, _flat(v), to, k_cache, v_cache)
-            _lib.check(_lib.load().dlrb200_qk_norm_rope(ctypes.byref(args), _stream_ptr(device.index)), "dlrb200_qk_norm_rope")
-    return (q_out, k_out) if return_keys else q_out
+        out = _native().qk_norm_rope_append(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), _heads(v, 4), slots.contiguous(),
+                                            k_cache, v_cache, float(eps), bool(interleaved), bool(return_keys))
+    return _result(out, "dlrb200_qk_norm_rope")
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------------
@@ -336,6 +293,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     are read on the device: a captured call follows them.  A table entry outside the caches counts as a page of zeros and
     is never followed.  Scores, softmax and sums are fp32.  No gradient.
     """
+    out = _native().paged_attention(q, k_cache, v_cache, block_table, lengths, scale)
+    if out is not None and type(out) is not int:
+        return out
     what = "paged_attention"
     _all_tensors(what, q, k_cache, v_cache, block_table, lengths)
     if q.dim() != 3:
@@ -360,16 +320,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
     device = _on_one_device(what, q, k_cache, v_cache, block_table, lengths)
     with torch.cuda.device(device):
-        lib = _lib.load()
-        out = torch.empty(n, heads, dim, dtype=q.dtype, device=device)
-        if n:
-            need = lib.dlrb200_paged_attention_workspace_bytes(heads, kv_heads, dim)
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            q = _heads(q, 2)
-            args = _lib.PagedAttentionArgs(
-                q.data_ptr(), *_strides(q), k_cache.data_ptr(), v_cache.data_ptr(), *k_cache.stride()[:3], *v_cache.stride()[:3],
-                block_table.data_ptr(), block_table.stride(0), lengths.data_ptr(), out.data_ptr(), workspace.data_ptr(), need,
-                n, heads, kv_heads, dim, block_table.shape[1], k_cache.shape[0], k_cache.shape[2], _TYPES[q.dtype],
-                1.0 / math.sqrt(dim) if scale is None else float(scale))
-            _lib.check(lib.dlrb200_paged_attention(ctypes.byref(args), _stream_ptr(device.index)), "dlrb200_paged_attention")
-    return out
+        out = _native().paged_attention(_heads(q, 2), k_cache, v_cache, block_table, lengths, None if scale is None else float(scale))
+    return _result(out, "dlrb200_paged_attention")

@@ -6,8 +6,8 @@ Every ``.cu`` under ``csrc/`` is compiled with
 ``-gencode arch=compute_100a,code=sm_100a -lineinfo`` and linked into
 ``libdlr_b200.so`` next to this file.  The CUDA runtime is linked statically,
 so the library does not depend on which runtime the host process loaded.
-``csrc/host.cpp`` becomes the Python module ``_host`` (walks over a net's
-parameters; see there).
+``csrc/host.cpp`` and ``csrc/host_attention.cpp`` become the Python module
+``_host`` (walks over a net's parameters, host side of the attention operators).
 """
 from __future__ import annotations
 
@@ -23,7 +23,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.normpath(os.path.join(HERE, "..", "csrc"))
 INCLUDE = os.path.normpath(os.path.join(HERE, "..", "..", "include"))
 LIB_PATH = os.path.join(HERE, "libdlr_b200.so")
-HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_attention.cpp")]
 OBJ_DIR = os.path.join(HERE, "build")
 
 NVCC_FLAGS = [
@@ -53,9 +53,9 @@ def _stale(target: str, deps) -> bool:
 
 def build_host(force: bool = False) -> str:
     """Compile the host-side helper module ``_host`` against torch's headers, if there is none for this Python and torch or
-    its source is newer."""
+    its sources are newer."""
     path = _lib.host_path()
-    if not force and not _stale(path, [HOST_SRC]):
+    if not force and not _stale(path, HOST_SRCS + [os.path.join(INCLUDE, "dlr_b200.h")]):
         return path
     import sysconfig
 
@@ -63,13 +63,14 @@ def build_host(force: bool = False) -> str:
     from torch.utils.cpp_extension import include_paths, library_paths
 
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"]]
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
+           "-I", INCLUDE, "-isystem", os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")]
     for p in include_paths():
         cmd += ["-isystem", p]
-    cmd += [HOST_SRC, "-o", path]
+    cmd += HOST_SRCS + ["-o", path]
     for p in library_paths():
         cmd += ["-L", p]
-    r = subprocess.run(cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10"], capture_output=True, text=True)
+    r = subprocess.run(cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("g++ failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     return path
