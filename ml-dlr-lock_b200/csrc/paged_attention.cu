@@ -32,7 +32,16 @@ constexpr int kWarpsA = 4;
 constexpr int kThreadsA = 32 * kWarpsA;
 constexpr int kUnit = 16;                        // tokens of a warp's step
 constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
-constexpr int kMostCtasPerSm = 2;
+// CTAs of an SM for heads of `dim`: as many as registers and shared memory allow.
+constexpr int ctas_per_sm(int dim) { return dim == 64 ? 4 : dim <= 128 ? 2 : 1; }
+constexpr int kMostCtasPerSm = 4;
+// Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (us):
+// 64 ragged requests of up to 8000 tokens, 8 heads of 128: 178 / 174 / 169 / 168; 200 of up to 1500, 12 heads of 64: 91 / 89
+// / 87 / 86; one of 131072, 8 heads: 93 / 92 / 95 / 98 where runs are 14 tiles and 9, 92 where they stay above 16.
+constexpr int kWaves = 4;
+constexpr int kLeastRun = 16;
+constexpr int kMostSms = 160;
+constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, int NT>
@@ -46,7 +55,7 @@ struct Shape {
     static constexpr int kJoin = kWarpsA * kRows * (D + 4) * 4;    // output of every warp, and its maxima and sums behind
     static constexpr int kJoinRow = D + 4;                         // floats; 16 bytes of padding
     static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kWarpsA * kRows * 8;
-    static constexpr int kCtasPerSm = kSmem <= 113 * 1024 ? 2 : 1;
+    static constexpr int kCtasPerSm = ctas_per_sm(D);
     static constexpr int kPart = kRows * (D + 2);                  // floats of a partial result: output, maxima, sums
 };
 
@@ -148,11 +157,17 @@ __device__ __forceinline__ long long scan_tiles(long long v, long long* scratch,
     return before + sum - v;
 }
 
-// Tiles per CTA for `total` tiles.
-__device__ __forceinline__ long long run_of(long long total, int ctas) {
-    const long long even = (total + ctas - 1) / ctas;
-    return even < 1 ? 1 : even;
-}
+// How the tiles are cut: into as many runs as CTAs are resident, or several times as many while runs stay long, so that SMs
+// that get more of the memory's bandwidth than others take more of them.
+struct Cut {
+    int resident, waves, least;          // CTAs, runs for each of them at most, tiles of a run if there is more than one for each
+
+    __device__ __forceinline__ long long run(long long total) const {
+        const long long fit = total / ((long long)resident * least);
+        const long long runs = (long long)resident * (fit < 1 ? 1 : fit < waves ? fit : waves), even = (total + runs - 1) / runs;
+        return even < 1 ? 1 : even;
+    }
+};
 
 // The request that holds tile `at`, and the tiles before it.
 struct Place {
@@ -161,7 +176,7 @@ struct Place {
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid_constant__ PagedAttention p, int groups) {
+__global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut) {
     using S = Shape<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long scratch[kWarpsA];
@@ -170,15 +185,18 @@ __global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid
     const int group_size = p.heads / p.kv_heads;
     const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
 
-    // all tiles, then the request in which this CTA's run begins
-    long long total = 0;
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    // all tiles, and the request in which this CTA's run begins
+    long long total = 0, mine = 0, before = 0;
     for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
         const int r = r0 + int(threadIdx.x);
         long long here;
-        scan_tiles<kWarpsA>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
+        mine = r < p.requests ? geo.tiles(r) : 0;
+        before = total + scan_tiles<kWarpsA>(mine, scratch, &here);
         total += here;
     }
-    const long long run = run_of(total, gridDim.x);
+    const long long run = cut.run(total);
     long long at = run * blockIdx.x;
     const long long end = at + run < total ? at + run : total;
     // requests without tokens belong to no tile: their zeros are written by the CTAs in turn
@@ -187,18 +205,22 @@ __global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid
             for (int i = threadIdx.x; i < p.heads * D / 2; i += kThreadsA)
                 reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + int64_t(r) * p.heads * D)[i] = 0;
     if (at >= end) return;
-    long long base = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
-        const int r = r0 + int(threadIdx.x);
-        const long long mine = r < p.requests ? geo.tiles(r) : 0;
-        long long here;
-        const long long before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
-        if (at >= before && at < before + mine) place = {r, before};
-        base += here;
+    if (p.requests <= kThreadsA) {
+        if (at >= before && at < before + mine) place = {int(threadIdx.x), before};
+    } else {
+        long long base = 0;
+        for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+            const int r = r0 + int(threadIdx.x);
+            mine = r < p.requests ? geo.tiles(r) : 0;
+            long long here;
+            before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
+            if (at >= before && at < before + mine) place = {r, before};
+            base += here;
+        }
     }
     __syncthreads();
     int request = place.request;
-    long long before = place.before;
+    before = place.before;
 
     const uint32_t ring = smem_u32(smem) + warp * (S::kStages * S::kStage);
     float* const join = reinterpret_cast<float*>(smem);
@@ -393,6 +415,7 @@ __global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid
             }
         }
         __syncthreads();
+        // (more than one CTA: the rest is joined by join_kernel)
         const bool whole = tile0 == 0 && tile1 == seg_tiles;
         float* const part = static_cast<float*>(p.workspace) + (int64_t(blockIdx.x) * 2 + (at == run * blockIdx.x ? 0 : 1)) * S::kPart;
         for (int i = threadIdx.x; i < rows * (D / 2); i += kThreadsA) {
@@ -428,15 +451,22 @@ __global__ void __launch_bounds__(kThreadsA) paged_attention_kernel(const __grid
     }
 }
 
-// One CTA per segment: joins the runs over which it was cut.
+// One CTA per query head: joins the runs over which its segment was cut.  It is launched while the first kernel still runs and
+// finds its place in the work meanwhile.  The factors of all parts come first, so that the loads of the parts do not wait for
+// one another; each warp adds up a quarter of them, in the order of the tokens.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreadsA) join_kernel(const __grid_constant__ PagedAttention p, int groups, int ctas) {
+__global__ void __launch_bounds__(kThreadsA) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut) {
     using S = Shape<D, NT>;
+    constexpr int kParts = kMostParts;           // of a segment: it takes no more runs than there are CTAs
     __shared__ long long scratch[kWarpsA];
     __shared__ long long before_us;
-    const int segments = p.kv_heads * groups;
-    const int request = blockIdx.x / segments, segment = blockIdx.x - request * segments;
-    const Geometry geo{p.lengths, p.requests, segments, (long long)p.columns << p.page_shift};
+    __shared__ float factor[kParts], highest[kWarpsA], sums[kWarpsA];
+    __shared__ float4 share[kWarpsA][D / 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int request = blockIdx.x / p.heads, head = blockIdx.x - request * p.heads;
+    const int group_size = p.heads / p.kv_heads, kv_head = head / group_size, in_group = head - kv_head * group_size;
+    const int segment = kv_head * groups + in_group / S::kRows, row = in_group % S::kRows;
+    const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
     long long total = 0;
     for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
         const int r = r0 + int(threadIdx.x);
@@ -447,33 +477,76 @@ __global__ void __launch_bounds__(kThreadsA) join_kernel(const __grid_constant__
     }
     __syncthreads();
     const int seg_tiles = (geo.tokens(request) + kTile - 1) / kTile;
-    if (seg_tiles == 0) return;
-    const long long run = run_of(total, ctas);
+    const long long run = cut.run(total);
     const long long begin = before_us + (long long)segment * seg_tiles, end = begin + seg_tiles;
-    const int cta0 = int(begin / run), cta1 = int((end - 1) / run);
-    if (cta0 == cta1) return;                   // not cut
-    const int group_size = p.heads / p.kv_heads, kv_head = segment / groups, group = segment - kv_head * groups;
-    const int head0 = kv_head * group_size + group * S::kRows, rows = min(S::kRows, group_size - group * S::kRows);
-    const float* const workspace = static_cast<const float*>(p.workspace);
+    const int cta0 = int(begin / run), parts = seg_tiles ? int((end - 1) / run) - cta0 + 1 : 0;
+    // The first CTA stays until the first kernel is done, whatever it has to do itself: this kernel then ends after that one,
+    // and what follows on the stream after both.
+    if (blockIdx.x == 0 || parts > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (parts <= 1) return;                     // not cut
     // the segment opens its CTA's run unless it begins inside it
-    auto part_of = [&](int c) { return workspace + (int64_t(c) * 2 + (begin <= run * c ? 0 : 1)) * S::kPart; };
-    for (int i = threadIdx.x; i < rows * (D / 2); i += kThreadsA) {
-        const int row = i / (D / 2), c = (i % (D / 2)) * 2;
-        float top = -INFINITY, sum = 0.f;
-        float2 v = make_float2(0.f, 0.f);
-        for (int cta = cta0; cta <= cta1; ++cta) {
-            const float* const part = part_of(cta);
-            const float2 ml = *reinterpret_cast<const float2*>(part + S::kRows * D + row * 2);
-            const float2 x = *reinterpret_cast<const float2*>(part + row * D + c);
-            const float next = fmaxf(top, ml.x), ref = next == -INFINITY ? 0.f : next;
-            const float f = exp2f(top - ref), g = exp2f(ml.x - ref);
-            top = next;
-            sum = sum * f + ml.y * g;
-            v.x = v.x * f + x.x * g;
-            v.y = v.y * f + x.y * g;
+    const int first_slot = begin <= run * cta0 ? 0 : 1;
+    const float* const workspace = static_cast<const float*>(p.workspace);
+    auto part_of = [&](int i) { return workspace + (int64_t(cta0 + i) * 2 + (i == 0 ? first_slot : 0)) * S::kPart; };
+
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += kThreadsA) {
+        factor[i] = part_of(i)[S::kRows * D + row * 2];
+        top = fmaxf(top, factor[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    if (lane == 0) highest[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarpsA; ++w) top = fmaxf(top, highest[w]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int i = threadIdx.x; i < parts; i += kThreadsA) {
+        factor[i] = exp2f(factor[i] - ref);
+        sum += factor[i] * part_of(i)[S::kRows * D + row * 2 + 1];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarpsA; ++w) sum += sums[w];
+
+    const int per = (parts + kWarpsA - 1) / kWarpsA, lo = warp * per, hi = min(parts, lo + per);
+#pragma unroll
+    for (int c0 = 0; c0 < D / 4; c0 += 32) {
+        const int c = c0 + lane;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < D / 4) {
+#pragma unroll 8
+            for (int i = lo; i < hi; ++i) {
+                const float2* const at = reinterpret_cast<const float2*>(part_of(i) + row * D + c * 4);
+                const float2 x = at[0], y = at[1];
+                const float f = factor[i];
+                v.x += f * x.x;
+                v.y += f * x.y;
+                v.z += f * y.x;
+                v.w += f * y.y;
+            }
+            share[warp][c] = v;
         }
-        const float inv = 1.f / sum;
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head0 + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
+    }
+    __syncthreads();
+    const float inv = 1.f / sum;
+    for (int c = threadIdx.x; c < D / 4; c += kThreadsA) {
+        float4 v = share[0][c];
+#pragma unroll
+        for (int w = 1; w < kWarpsA; ++w) {
+            const float4 x = share[w][c];
+            v.x += x.x;
+            v.y += x.y;
+            v.z += x.z;
+            v.w += x.w;
+        }
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head) * D + c * 4) =
+            make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
     }
 }
 
@@ -484,10 +557,22 @@ cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
     const int group_size = a.heads / a.kv_heads, groups = (group_size + S::kRows - 1) / S::kRows;
-    const int ctas = S::kCtasPerSm * num_sms;
-    kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups);
-    join_kernel<T, D, NT><<<unsigned(a.requests) * a.kv_heads * groups, kThreadsA, 0, stream>>>(a, groups, ctas);
-    return cudaGetLastError();
+    // no more CTAs than the table could hold tiles
+    const long long most = (long long)a.requests * a.kv_heads * groups * (((long long)a.columns << a.page_shift) / kTile + 1);
+    Cut cut{S::kCtasPerSm * min(num_sms, kMostSms), kWaves, kLeastRun};
+    if (most < cut.resident) cut.resident = int(most);
+    const int ctas = cut.resident * kWaves;
+    kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups, cut);
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.requests) * unsigned(a.heads));
+    cfg.blockDim = dim3(kThreadsA);
+    cfg.stream = stream;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, groups, cut);
 }
 
 template <typename T, int D>
@@ -514,7 +599,7 @@ bool paged_attention_supported(int heads, int kv_heads, int dim) {
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int dim, int num_sms) {
     const int rows = heads / kv_heads <= 8 ? 8 : 16;
-    return size_t(kMostCtasPerSm) * num_sms * 2 * rows * (dim + 2) * sizeof(float);
+    return size_t(ctas_per_sm(dim)) * (num_sms < kMostSms ? num_sms : kMostSms) * kWaves * 2 * rows * (dim + 2) * sizeof(float);
 }
 
 cudaError_t paged_attention(const PagedAttention& a, int num_sms, cudaStream_t stream) {
