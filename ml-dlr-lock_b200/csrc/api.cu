@@ -806,7 +806,7 @@ int dlrb200_qk_norm_rope(const dlrb200_norm_rope_args* s, void* stream) {
     a.tokens = s->tokens, a.q_heads = s->q_heads, a.k_heads = s->k_heads, a.dim = s->dim, a.half = s->half, a.table_rows = s->table_rows;
     a.f16 = s->type == DLRB200_F16, a.weights_f32 = s->weights_f32 != 0, a.positions_64 = s->positions_64 != 0;
     a.interleaved = s->interleaved != 0, a.eps = s->eps;
-    return cuda_ok(dlr::norm_rope(a, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
+    return cuda_ok(dlr::norm_rope(a, di.num_sms, static_cast<cudaStream_t>(stream))) ? DLRB200_OK : DLRB200_ERR_CUDA;
 }
 
 size_t dlrb200_qk_norm_rope_backward_workspace_bytes(int dim) {

@@ -53,7 +53,7 @@ struct NormRopeBackward {
 };
 
 int norm_rope_partials(int num_sms);
-cudaError_t norm_rope(const NormRope& a, cudaStream_t stream);
+cudaError_t norm_rope(const NormRope& a, int num_sms, cudaStream_t stream);
 cudaError_t norm_rope_backward(const NormRopeBackward& a, int num_sms, cudaStream_t stream);
 
 }  // namespace dlr
