@@ -757,7 +757,7 @@ int shape_of_heads(int q_heads, int k_heads, int dim, int half) {
 int dlrb200_paged_plan(const dlrb200_plan_step* s, void* stream) {
     if (!s || s->requests < 0 || s->columns < 0 || s->pages < 0 || s->width < 0 || s->rows < 0) return DLRB200_ERR_INVALID_ARG;
     const int shift = page_shift_of(s->page_size);
-    if (shift < 0 || s->requests > DLRB200_MAX_PLAN_REQUESTS || (int64_t(s->pages) << shift) > 0x7fffffff) return DLRB200_ERR_UNSUPPORTED_SHAPE;
+    if (shift < 0 || s->requests > DLRB200_MAX_PLAN_REQUESTS || s->rows > (1 << 30) || (int64_t(s->pages) << shift) > 0x7fffffff) return DLRB200_ERR_UNSUPPORTED_SHAPE;
     if (s->width > 0 && int64_t(s->width) * s->requests != s->rows) return DLRB200_ERR_INVALID_ARG;
     if (!s->n_free || !s->starts || !s->n_free_out || (s->rows > 0 && (!s->slots || !s->positions)) || (s->pages > 0 && !s->free_pages) ||
         (s->requests > 0 && (!s->lengths || !s->new_tokens || !s->lengths_out || (s->columns > 0 && !s->block_table))))

@@ -51,7 +51,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-constexpr int64_t kMostInt = std::numeric_limits<int>::max();
+constexpr int64_t kMostInt = std::numeric_limits<int>::max(), kMostRows = int64_t(1) << 30;
 
 // The tensor behind an argument; null for anything else.
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -139,10 +139,10 @@ PyObject* paged_plan(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
         pages->size(0) > kMostInt / page_size)
         Py_RETURN_NONE;
     if (o[6] != Py_None) {
-        if (!integer(o[6], &width) || width < 1 || width > kMostInt || width * n > kMostInt) Py_RETURN_NONE;
+        if (!integer(o[6], &width) || width < 1 || width > kMostInt || width * n > kMostRows) Py_RETURN_NONE;
         if (o[7] != Py_None && (!integer(o[7], &rows) || rows != width * n)) Py_RETURN_NONE;
         rows = width * n;
-    } else if (!integer(o[7], &rows) || rows < 0 || rows > kMostInt) {
+    } else if (!integer(o[7], &rows) || rows < 0 || rows > kMostRows) {
         Py_RETURN_NONE;
     }
     at::Tensor slots, positions, starts, lengths_out, count_out;

@@ -167,8 +167,8 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
         if type(width) is not int or width < 1:
             raise ValueError(f"{what}: width is an int, at least 1")
         rows = width * n
-    if type(rows) is not int or rows < 0 or rows > 0x7fffffff:
-        raise ValueError(f"{what}: {rows} rows")
+    if type(rows) is not int or rows < 0 or rows > 1 << 30:
+        raise ValueError(f"{what}: {rows} rows, 0 to 2^30 are possible")
     device = _on_one_device(what, lengths, new_tokens, block_table, free_pages, n_free, finished)
     with torch.cuda.device(device):
         out = _native().paged_plan(lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
