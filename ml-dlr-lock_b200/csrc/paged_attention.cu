@@ -30,6 +30,8 @@ namespace {
 
 constexpr int kWarpsA = 4;
 constexpr int kThreadsA = 32 * kWarpsA;
+constexpr int kWarpsJ = 8;                       // of the joining kernel
+constexpr int kThreadsJ = 32 * kWarpsJ;
 constexpr int kUnit = 16;                        // tokens of a warp's step
 constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
 // CTAs of an SM for heads of `dim`: as many as registers and shared memory allow.
@@ -56,11 +58,12 @@ struct Shape {
     static constexpr int kJoinRow = D + 4;                         // floats; 16 bytes of padding
     static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kWarpsA * kRows * 8;
     static constexpr int kCtasPerSm = ctas_per_sm(D);
-    static constexpr int kPart = kRows * (D + 2);                  // floats of a partial result: output, maxima, sums
+    static constexpr int kPart = kRows * (D + 2);                      // floats of a partial result: output, maxima, sums
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// (the hint: keys and values go first from L2, and leave the partial results there)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes, uint64_t hint) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes), "l"(hint) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -226,6 +229,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
     float* const join = reinterpret_cast<float*>(smem);
     float2* const join_ml = reinterpret_cast<float2*>(smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin));
     const float scale = p.scale * kLog2e;
+    const uint64_t hint = l2_policy_evict_first();
 
     for (; at < end;) {
         // the segment that holds tile `at`
@@ -276,14 +280,14 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                     const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
                     const uint32_t bytes = row < valid ? 16 : 0;
                     const int slot = row < valid ? slot0 + row : 0;
-                    cp_async16(stage + row * S::kRow + col * 16, k + slot * p.k_slot + col * 8, bytes);
+                    cp_async16(stage + row * S::kRow + col * 16, k + slot * p.k_slot + col * 8, bytes, hint);
                 }
 #pragma unroll
                 for (int i = 0; i < kUnit * kChunks / 32; ++i) {
                     const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
                     const uint32_t bytes = row < valid ? 16 : 0;
                     const int slot = row < valid ? slot0 + row : 0;
-                    cp_async16(stage + S::kHalf + row * S::kRow + col * 16, v + slot * p.v_slot + col * 8, bytes);
+                    cp_async16(stage + S::kHalf + row * S::kRow + col * 16, v + slot * p.v_slot + col * 8, bytes, hint);
                 }
             }
             cp_async_commit();
@@ -451,102 +455,161 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
     }
 }
 
-// One CTA per query head: joins the runs over which its segment was cut.  It is launched while the first kernel still runs and
-// finds its place in the work meanwhile.  The factors of all parts come first, so that the loads of the parts do not wait for
-// one another; each warp adds up a quarter of them, in the order of the tokens.
+// Where a head's partial results are: `parts` of them, in the slots of runs `run`, run + 1, ...
+struct Pieces {
+    int parts, run, first_slot, request, head, row;
+};
+
+// Joins the runs over which segments were cut: `per_cta` (1 or 8) query heads to a CTA.  It is launched while the first kernel
+// still runs and finds its place in the work meanwhile.  A warp joins a head of few parts by itself, all warps of the CTA one of
+// many; maxima come first, so that the loads of the parts do not wait for one another.  Sums run in the order of the tokens.
+// (Measured behind the first kernel, us: 6 for 64 heads of 108 parts each.)
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreadsA) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut) {
+__global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut, int per_cta) {
     using S = Shape<D, NT>;
-    constexpr int kParts = kMostParts;           // of a segment: it takes no more runs than there are CTAs
-    __shared__ long long scratch[kWarpsA];
-    __shared__ long long before_us;
-    __shared__ float factor[kParts], highest[kWarpsA], sums[kWarpsA];
-    __shared__ float4 share[kWarpsA][D / 4];
+    constexpr int kColumns = (D / 4 + 31) / 32;          // of four values, per lane
+    constexpr int kBatch = 16 / kColumns;                // loads in flight
+    constexpr int kFew = 16;
+    __shared__ long long scratch[kWarpsJ], before[kWarpsJ];
+    __shared__ Pieces found[kWarpsJ];
+    __shared__ float2 ml[kMostParts];
+    __shared__ float highest[kWarpsJ], sums[kWarpsJ];
+    __shared__ float4 share[kWarpsJ][D / 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int request = blockIdx.x / p.heads, head = blockIdx.x - request * p.heads;
-    const int group_size = p.heads / p.kv_heads, kv_head = head / group_size, in_group = head - kv_head * group_size;
-    const int segment = kv_head * groups + in_group / S::kRows, row = in_group % S::kRows;
+    const int group_size = p.heads / p.kv_heads, first_head = int(blockIdx.x) * per_cta, all_heads = p.requests * p.heads;
     const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
+    const int first_request = first_head / p.heads;
     long long total = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+    for (int r0 = 0; r0 < p.requests; r0 += kThreadsJ) {
         const int r = r0 + int(threadIdx.x);
         long long here;
-        const long long before = total + scan_tiles<kWarpsA>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
-        if (r == request) before_us = before;
+        const long long at = total + scan_tiles<kWarpsJ>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
+        if (r >= first_request && r < first_request + per_cta) before[r - first_request] = at;
         total += here;
     }
     __syncthreads();
-    const int seg_tiles = (geo.tokens(request) + kTile - 1) / kTile;
-    const long long run = cut.run(total);
-    const long long begin = before_us + (long long)segment * seg_tiles, end = begin + seg_tiles;
-    const int cta0 = int(begin / run), parts = seg_tiles ? int((end - 1) / run) - cta0 + 1 : 0;
+    Pieces mine{};
+    if (warp < per_cta && first_head + warp < all_heads) {
+        const int request = (first_head + warp) / p.heads, head = first_head + warp - request * p.heads;
+        const int kv_head = head / group_size, in_group = head - kv_head * group_size;
+        const int segment = kv_head * groups + in_group / S::kRows;
+        const int seg_tiles = (geo.tokens(request) + kTile - 1) / kTile;
+        if (seg_tiles) {
+            const long long run = cut.run(total), begin = before[request - first_request] + (long long)segment * seg_tiles;
+            const int first = int(begin / run), last = int((begin + seg_tiles - 1) / run);
+            // the segment opens its first run unless it begins inside it
+            mine = {last - first + 1, first, begin <= run * first ? 0 : 1, request, head, in_group % S::kRows};
+        }
+    }
+    if (lane == 0) found[warp] = mine;
     // The first CTA stays until the first kernel is done, whatever it has to do itself: this kernel then ends after that one,
     // and what follows on the stream after both.
-    if (blockIdx.x == 0 || parts > 1) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (parts <= 1) return;                     // not cut
-    // the segment opens its CTA's run unless it begins inside it
-    const int first_slot = begin <= run * cta0 ? 0 : 1;
+    const bool any = __syncthreads_or(mine.parts > 1);
+    if (blockIdx.x == 0 || any) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!any) return;                                    // nothing was cut
+
     const float* const workspace = static_cast<const float*>(p.workspace);
-    auto part_of = [&](int i) { return workspace + (int64_t(cta0 + i) * 2 + (i == 0 ? first_slot : 0)) * S::kPart; };
-
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += kThreadsA) {
-        factor[i] = part_of(i)[S::kRows * D + row * 2];
-        top = fmaxf(top, factor[i]);
-    }
+    auto part_of = [&](const Pieces& a, int i) { return workspace + (int64_t(a.run + i) * 2 + (i == 0 ? a.first_slot : 0)) * S::kPart; };
+    auto ml_of = [&](const Pieces& a, int i) { return *reinterpret_cast<const float2*>(part_of(a, i) + S::kRows * D + a.row * 2); };
+    // this lane's columns of a part's row
+    auto load = [&](const Pieces& a, int i, bool real, float4 (&x)[kColumns]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    if (lane == 0) highest[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWarpsA; ++w) top = fmaxf(top, highest[w]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = threadIdx.x; i < parts; i += kThreadsA) {
-        factor[i] = exp2f(factor[i] - ref);
-        sum += factor[i] * part_of(i)[S::kRows * D + row * 2 + 1];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarpsA; ++w) sum += sums[w];
-
-    const int per = (parts + kWarpsA - 1) / kWarpsA, lo = warp * per, hi = min(parts, lo + per);
-#pragma unroll
-    for (int c0 = 0; c0 < D / 4; c0 += 32) {
-        const int c = c0 + lane;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < D / 4) {
-#pragma unroll 8
-            for (int i = lo; i < hi; ++i) {
-                const float2* const at = reinterpret_cast<const float2*>(part_of(i) + row * D + c * 4);
-                const float2 x = at[0], y = at[1];
-                const float f = factor[i];
-                v.x += f * x.x;
-                v.y += f * x.y;
-                v.z += f * y.x;
-                v.w += f * y.y;
-            }
-            share[warp][c] = v;
+        for (int k = 0; k < kColumns; ++k) {
+            const int c = k * 32 + lane;
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (real && c < D / 4) x[k] = *reinterpret_cast<const float4*>(part_of(a, i) + a.row * D + c * 4);
         }
-    }
-    __syncthreads();
-    const float inv = 1.f / sum;
-    for (int c = threadIdx.x; c < D / 4; c += kThreadsA) {
-        float4 v = share[0][c];
+    };
+    auto add = [](float4 (&v)[kColumns], float f, const float4 (&x)[kColumns]) {
 #pragma unroll
-        for (int w = 1; w < kWarpsA; ++w) {
-            const float4 x = share[w][c];
-            v.x += x.x;
-            v.y += x.y;
-            v.z += x.z;
-            v.w += x.w;
+        for (int k = 0; k < kColumns; ++k) {
+            v[k].x += f * x[k].x;
+            v[k].y += f * x[k].y;
+            v[k].z += f * x[k].z;
+            v[k].w += f * x[k].w;
         }
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head) * D + c * 4) =
+    };
+    auto write = [&](const Pieces& a, int c, float4 v, float inv) {
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (int64_t(a.request) * p.heads + a.head) * D + c * 4) =
             make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+    };
+    auto warp_max = [](float x) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
+        return x;
+    };
+    auto warp_sum = [](float x) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+        return x;
+    };
+
+    if (mine.parts > 1 && mine.parts <= kFew) {
+        const float2 m = lane < mine.parts ? ml_of(mine, lane) : make_float2(-INFINITY, 0.f);
+        const float top = warp_max(m.x), f = exp2f(m.x - (top == -INFINITY ? 0.f : top)), sum = warp_sum(f * m.y);
+        float4 v[kColumns] = {};
+        for (int i0 = 0; i0 < mine.parts; i0 += kBatch) {
+            float4 x[kBatch][kColumns];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) load(mine, i0 + i, i0 + i < mine.parts, x[i]);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) add(v, __shfl_sync(~0u, f, (i0 + i) & 31), x[i]);      // (0 behind the last part)
+        }
+#pragma unroll
+        for (int k = 0; k < kColumns; ++k)
+            if (k * 32 + lane < D / 4) write(mine, k * 32 + lane, v[k], 1.f / sum);
+    }
+    for (int w = 0; w < per_cta; ++w) {
+        const Pieces a = found[w];
+        if (a.parts <= kFew) continue;
+        float top = -INFINITY;
+        for (int i = threadIdx.x; i < a.parts; i += kThreadsJ) {
+            ml[i] = ml_of(a, i);
+            top = fmaxf(top, ml[i].x);
+        }
+        top = warp_max(top);
+        if (lane == 0) highest[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kWarpsJ; ++k) top = fmaxf(top, highest[k]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const int per = (a.parts + kWarpsJ - 1) / kWarpsJ, lo = warp * per, hi = min(a.parts, lo + per);
+        float4 v[kColumns] = {};
+        float sum = 0.f;
+        for (int i0 = lo; i0 < hi; i0 += kBatch) {
+            float4 x[kBatch][kColumns];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) load(a, i0 + i, i0 + i < hi, x[i]);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const float2 m = i0 + i < hi ? ml[i0 + i] : make_float2(-INFINITY, 0.f);
+                const float f = exp2f(m.x - ref);
+                sum += f * m.y;
+                add(v, f, x[i]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kColumns; ++k)
+            if (k * 32 + lane < D / 4) share[warp][k * 32 + lane] = v[k];
+        if (lane == 0) sums[warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kWarpsJ; ++k) sum += sums[k];
+        const float inv = 1.f / sum;
+        for (int c = threadIdx.x; c < D / 4; c += kThreadsJ) {
+            float4 x = share[0][c];
+#pragma unroll
+            for (int k = 1; k < kWarpsJ; ++k) {
+                const float4 y = share[k][c];
+                x.x += y.x;
+                x.y += y.y;
+                x.z += y.z;
+                x.w += y.w;
+            }
+            write(a, c, x, inv);
+        }
+        __syncthreads();                                 // the next head's turn
     }
 }
 
@@ -567,12 +630,14 @@ cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.requests) * unsigned(a.heads));
-    cfg.blockDim = dim3(kThreadsA);
+    // a head to a CTA while that is a few CTAs for each SM at most
+    const int per_cta = int64_t(a.requests) * a.heads <= 4 * num_sms ? 1 : kWarpsJ;
+    cfg.gridDim = dim3((unsigned(a.requests) * unsigned(a.heads) + per_cta - 1) / per_cta);
+    cfg.blockDim = dim3(kThreadsJ);
     cfg.stream = stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, groups, cut);
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, groups, cut, per_cta);
 }
 
 template <typename T, int D>
