@@ -11,12 +11,12 @@
 // one request and head).  What is cut is joined by a second, small kernel from partial results in fp32, in the order of the
 // tokens, so that results repeat bit for bit; what is whole is finished by its CTA.
 //
-// A warp takes 16 tokens of a tile at a time, on its own: it copies their keys and values to its own ring in shared memory
-// (cp.async, rows padded by 16 bytes so that ldmatrix meets no bank twice), multiplies with mma.sync, and keeps maximum, sum
-// and output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  The 16 rows of the
-// instruction hold up to 16 heads that share the keys; with up to eight, rows 8 to 15 of the second product hold what the
-// rounding of the softmax weights to 16 bits left over, so that weights count with twice the bits at no cost (with more, a
-// second instruction does that).
+// A warp takes 16 tokens of a tile at a time, on its own: it copies their keys and their values to its own ring in shared memory
+// (cp.async, rows padded by 16 bytes so that ldmatrix meets no bank twice), multiplies with mma.sync, and keeps maximum, sum and
+// output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  Scores are (heads x tokens), the
+// output is turned round, (values x heads): the scores' registers then are the second product's operand as they are, and the
+// output of eight heads takes half the registers that 16 rows would.  Softmax weights enter that product as the sum of two 16-bit
+// terms, so that their rounding (2^-16) does not show in the result.
 #include "paged_attention.h"
 
 #include <cuda_bf16.h>
@@ -34,9 +34,11 @@ constexpr int kWarpsJ = 8;                       // of the joining kernel
 constexpr int kThreadsJ = 32 * kWarpsJ;
 constexpr int kUnit = 16;                        // tokens of a warp's step
 constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
-// CTAs of an SM for heads of `dim`: as many as registers and shared memory allow.
-constexpr int ctas_per_sm(int dim) { return dim == 64 ? 4 : dim <= 128 ? 2 : 1; }
-constexpr int kMostCtasPerSm = 4;
+// CTAs of an SM for heads of `dim`, nt groups of eight sharing keys: as many as registers and shared memory allow.  More warps
+// count for more than more copies in flight: a warp's step is a chain of dependent instructions (460 MB, us: 6 heads of 128 with
+// 3 CTAs of 3 or 4 halves 77, 2 CTAs of 5 or 6 halves 80; 3 heads of 256 with 2 CTAs of 2 halves 76, of 3 halves 80, one CTA of 4 85).
+constexpr int ctas_per_sm(int dim, int nt) { return dim == 64 ? (nt == 1 ? 5 : 4) : dim == 96 ? (nt == 1 ? 4 : 3) : dim == 128 ? 3 : 2; }
+constexpr int kMostCtasPerSm = 5;
 // Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (us):
 // 64 ragged requests of up to 8000 tokens, 8 heads of 128: 178 / 174 / 169 / 168; 200 of up to 1500, 12 heads of 64: 91 / 89
 // / 87 / 86; one of 131072, 8 heads: 93 / 92 / 95 / 98 where runs are 14 tiles and 9, 92 where they stay above 16.
@@ -50,15 +52,14 @@ template <int D, int NT>
 struct Shape {
     static constexpr int kRow = D * 2 + 16;                        // bytes of a row in shared memory
     static constexpr int kHalf = kUnit * kRow;                     // keys (or values) of a step
-    static constexpr int kStage = 2 * kHalf;
-    static constexpr int kStages = D <= 128 ? 3 : 2;
-    static constexpr int kRing = kWarpsA * kStages * kStage;
+    static constexpr int kHalves = D <= 128 ? 3 : 2;               // of a warp's ring
+    static constexpr int kRing = kWarpsA * kHalves * kHalf;
     static constexpr int kRows = 8 * NT;                           // query heads of a segment
-    static constexpr int kJoin = kWarpsA * kRows * (D + 4) * 4;    // output of every warp, and its maxima and sums behind
-    static constexpr int kJoinRow = D + 4;                         // floats; 16 bytes of padding
+    static constexpr int kJoinRow = D + 4;                         // floats; the padding keeps banks apart
+    static constexpr int kJoin = kWarpsA * kRows * kJoinRow * 4;   // output of every warp; its maxima and sums lie behind
     static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kWarpsA * kRows * 8;
-    static constexpr int kCtasPerSm = ctas_per_sm(D);
-    static constexpr int kPart = kRows * (D + 2);                      // floats of a partial result: output, maxima, sums
+    static constexpr int kCtasPerSm = ctas_per_sm(D, NT);
+    static constexpr int kPart = kRows * (D + 2);                  // floats of a partial result: output, maxima, sums
 };
 
 // (the hint: keys and values go first from L2, and leave the partial results there)
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
     int request = place.request;
     before = place.before;
 
-    const uint32_t ring = smem_u32(smem) + warp * (S::kStages * S::kStage);
+    const uint32_t ring = smem_u32(smem) + warp * (S::kHalves * S::kHalf);
     float* const join = reinterpret_cast<float*>(smem);
     float2* const join_ml = reinterpret_cast<float2*>(smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin));
     const float scale = p.scale * kLog2e;
@@ -264,36 +265,33 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
             if (s < steps) id = table[((first + s * kWarpsA) * kUnit) >> p.page_shift];
             page_ids = id;
         };
-        auto fetch = [&](int step) {
+        // copies half n of the steps: the keys of step n / 2, or its values
+        int in = 0;
+        auto fetch = [&](int n) {
+            const int step = n >> 1;
             if (step < steps) {
-                if ((step & 31) == 0) load_pages(step);
+                if ((n & 63) == 0) load_pages(step);
                 const int page = __shfl_sync(~0u, page_ids, step & 31);
                 const int token0 = (first + step * kWarpsA) * kUnit;
                 const int slot0 = token0 & ((1 << p.page_shift) - 1);
                 const int valid = unsigned(page) < unsigned(p.pages) ? min(kUnit, tokens - token0) : 0;
-                const T* const k = k_head + (valid ? page : 0) * p.k_page;
-                const T* const v = v_head + (valid ? page : 0) * p.v_page;
-                const uint32_t stage = ring + (step % S::kStages) * S::kStage;
+                const T* const src = (n & 1 ? v_head + (valid ? page : 0) * p.v_page : k_head + (valid ? page : 0) * p.k_page);
+                const int64_t slot_stride = n & 1 ? p.v_slot : p.k_slot;
+                const uint32_t stage = ring + in * S::kHalf;
                 constexpr int kChunks = D / 8;
 #pragma unroll
                 for (int i = 0; i < kUnit * kChunks / 32; ++i) {
                     const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
                     const uint32_t bytes = row < valid ? 16 : 0;
                     const int slot = row < valid ? slot0 + row : 0;
-                    cp_async16(stage + row * S::kRow + col * 16, k + slot * p.k_slot + col * 8, bytes, hint);
-                }
-#pragma unroll
-                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
-                    const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
-                    const uint32_t bytes = row < valid ? 16 : 0;
-                    const int slot = row < valid ? slot0 + row : 0;
-                    cp_async16(stage + S::kHalf + row * S::kRow + col * 16, v + slot * p.v_slot + col * 8, bytes, hint);
+                    cp_async16(stage + row * S::kRow + col * 16, src + slot * slot_stride + col * 8, bytes, hint);
                 }
             }
             cp_async_commit();
+            in = in + 1 == S::kHalves ? 0 : in + 1;
         };
 #pragma unroll
-        for (int s = 0; s < S::kStages - 1; ++s) fetch(s);
+        for (int n = 0; n < S::kHalves - 1; ++n) fetch(n);
 
         // queries: row lane / 4 (and + 8), as the first operand of the products with 16 values each
         uint32_t q[D / 16][2 * NT];
@@ -315,47 +313,59 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 }
         }
 
-        float o[D / 8][4], m[NT], l[NT];
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+        // output, turned round: 16 values of a head times 8 heads to a tile
+        float o[NT][D / 16][4], m[NT], l[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][t][i] = 0.f;
             m[n] = -INFINITY;
             l[n] = 0.f;
         }
 
+        // both products take 8 x 8 blocks of a stage in the same order: tokens 0-7 and 8-15, of each two runs of eight values
+        const uint32_t in_stage = ((lane & 7) + ((lane >> 4) & 1) * 8) * S::kRow + ((lane >> 3) & 1) * 16;
+        int at_half = 0;
+        auto next_half = [&](int n) {
+            cp_async_wait<S::kHalves - 2>();
+            __syncwarp();                       // the half's copies are there, and every lane is done with the one before
+            fetch(n + S::kHalves - 1);
+            const uint32_t stage = ring + at_half * S::kHalf + in_stage;
+            at_half = at_half + 1 == S::kHalves ? 0 : at_half + 1;
+            return stage;
+        };
         for (int step = 0; step < steps; ++step) {
-            cp_async_wait<S::kStages - 2>();
-            __syncwarp();                       // the step's copies are there, and every lane is done with the step before
-            fetch(step + S::kStages - 1);
-            const uint32_t stage = ring + (step % S::kStages) * S::kStage;
-            // scores of 16 tokens: two products of 8 tokens each
-            float s[2][4];
+            // scores of 16 tokens: two products of 8 tokens each, in two chains
+            const uint32_t k_at = next_half(2 * step);
+            float s[2][2][4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
-            const uint32_t k_at = stage + ((lane & 7) + ((lane >> 4) & 1) * 8) * S::kRow + ((lane >> 3) & 1) * 16;
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[c][n][i] = 0.f;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
                 uint32_t b0, b1, b2, b3;
                 ldmatrix_x4(k_at + k * 32, b0, b1, b2, b3);
                 if constexpr (NT == 1) {
-                    mma16816<T>(s[0], q[k][0], 0u, q[k][1], 0u, b0, b1);
-                    mma16816<T>(s[1], q[k][0], 0u, q[k][1], 0u, b2, b3);
+                    mma16816<T>(s[k & 1][0], q[k][0], 0u, q[k][1], 0u, b0, b1);
+                    mma16816<T>(s[k & 1][1], q[k][0], 0u, q[k][1], 0u, b2, b3);
                 } else {
-                    mma16816<T>(s[0], q[k][0], q[k][1], q[k][2], q[k][3], b0, b1);
-                    mma16816<T>(s[1], q[k][0], q[k][1], q[k][2], q[k][3], b2, b3);
+                    mma16816<T>(s[k & 1][0], q[k][0], q[k][1], q[k][2], q[k][3], b0, b1);
+                    mma16816<T>(s[k & 1][1], q[k][0], q[k][1], q[k][2], q[k][3], b2, b3);
                 }
             }
             const int valid = tokens - (first + step * kWarpsA) * kUnit;
             float alpha[NT];
-            uint32_t hi[2 * NT], lo[2 * NT];
+            uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float x[4] = {s[0][2 * n] * scale, s[0][2 * n + 1] * scale, s[1][2 * n] * scale, s[1][2 * n + 1] * scale};
+                float x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = (s[0][i >> 1][2 * n + (i & 1)] + s[1][i >> 1][2 * n + (i & 1)]) * scale;
                 if (valid < kUnit) {
                     const int t = (lane % 4) * 2;
                     if (t >= valid) x[0] = -INFINITY;
@@ -370,52 +380,51 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - ref);
                 l[n] = l[n] * alpha[n] + ((x[0] + x[1]) + (x[2] + x[3]));
-                split2<T>(x[0], x[1], hi[n], lo[n]);
-                split2<T>(x[2], x[3], hi[NT + n], lo[NT + n]);
+                split2<T>(x[0], x[1], hi[n][0], lo[n][0]);
+                split2<T>(x[2], x[3], hi[n][1], lo[n][1]);
             }
             bool same = alpha[0] == 1.f;
             if constexpr (NT == 2) same = same && alpha[1] == 1.f;
             if (!__all_sync(~0u, same)) {
 #pragma unroll
-                for (int n = 0; n < D / 8; ++n) {
-                    o[n][0] *= alpha[0];
-                    o[n][1] *= alpha[0];
-                    o[n][2] *= alpha[NT - 1];
-                    o[n][3] *= alpha[NT - 1];
+                for (int n = 0; n < NT; ++n) {
+                    // of the two heads whose values this lane holds
+                    const float a0 = __shfl_sync(~0u, alpha[n], (lane % 4) * 8), a1 = __shfl_sync(~0u, alpha[n], (lane % 4) * 8 + 4);
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t) {
+                        o[n][t][0] *= a0;
+                        o[n][t][1] *= a1;
+                        o[n][t][2] *= a0;
+                        o[n][t][3] *= a1;
+                    }
                 }
             }
-            const uint32_t v_at = stage + S::kHalf + ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kRow + ((lane >> 4) & 1) * 16;
+            const uint32_t v_at = next_half(2 * step + 1);
 #pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-                uint32_t b0, b1, b2, b3;
-                ldmatrix_x4_trans(v_at + n * 32, b0, b1, b2, b3);
-                if constexpr (NT == 1) {
-                    mma16816<T>(o[2 * n], hi[0], lo[0], hi[1], lo[1], b0, b1);
-                    mma16816<T>(o[2 * n + 1], hi[0], lo[0], hi[1], lo[1], b2, b3);
-                } else {
-                    mma16816<T>(o[2 * n], hi[0], hi[1], hi[2], hi[3], b0, b1);
-                    mma16816<T>(o[2 * n + 1], hi[0], hi[1], hi[2], hi[3], b2, b3);
-                    mma16816<T>(o[2 * n], lo[0], lo[1], lo[2], lo[3], b0, b1);
-                    mma16816<T>(o[2 * n + 1], lo[0], lo[1], lo[2], lo[3], b2, b3);
-                }
+            for (int t = 0; t < D / 16; ++t) {
+                uint32_t a0, a1, a2, a3;
+                ldmatrix_x4_trans(v_at + t * 32, a0, a1, a2, a3);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, lo[n][0], lo[n][1]);
             }
         }
         cp_async_wait<0>();
         __syncthreads();                        // the rings are free
 
-        // the warps' results: maxima and sums, outputs (both halves of the weights added up)
+        // the warps' results: maxima and sums, outputs
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const float sum = quad_sum(l[n]);
-            const int row = lane / 4 + 8 * n;
-            if (lane % 4 == 0) join_ml[warp * S::kRows + row] = make_float2(m[n], sum);
-            float* const at_row = join + (warp * S::kRows + row) * S::kJoinRow + (lane % 4) * 2;
+            if (lane % 4 == 0) join_ml[warp * S::kRows + lane / 4 + 8 * n] = make_float2(m[n], sum);
+            float* const at_head = join + (warp * S::kRows + (lane % 4) * 2 + 8 * n) * S::kJoinRow + lane / 4;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                float2 v;
-                if constexpr (NT == 1) v = make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
-                else v = make_float2(o[c][2 * n], o[c][2 * n + 1]);
-                *reinterpret_cast<float2*>(at_row + c * 8) = v;
+            for (int t = 0; t < D / 16; ++t) {
+                at_head[t * 16] = o[n][t][0];
+                at_head[t * 16 + S::kJoinRow] = o[n][t][1];
+                at_head[t * 16 + 8] = o[n][t][2];
+                at_head[t * 16 + 8 + S::kJoinRow] = o[n][t][3];
             }
         }
         __syncthreads();
@@ -664,7 +673,7 @@ bool paged_attention_supported(int heads, int kv_heads, int dim) {
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int dim, int num_sms) {
     const int rows = heads / kv_heads <= 8 ? 8 : 16;
-    return size_t(ctas_per_sm(dim)) * (num_sms < kMostSms ? num_sms : kMostSms) * kWaves * 2 * rows * (dim + 2) * sizeof(float);
+    return size_t(ctas_per_sm(dim, heads / kv_heads <= 8 ? 1 : 2)) * (num_sms < kMostSms ? num_sms : kMostSms) * kWaves * 2 * rows * (dim + 2) * sizeof(float);
 }
 
 cudaError_t paged_attention(const PagedAttention& a, int num_sms, cudaStream_t stream) {
