@@ -854,7 +854,7 @@ int dlrb200_paged_attention(const dlrb200_paged_attention_args* s, void* stream)
     if (!s || s->requests < 0 || s->columns < 0 || s->pages < 0 || (s->type != DLRB200_BF16 && s->type != DLRB200_F16)) return DLRB200_ERR_INVALID_ARG;
     const int shift = page_shift_of(s->page_size);
     if (shift < 0 || !dlr::paged_attention_supported(s->heads, s->kv_heads, s->dim) || int64_t(s->requests) * s->heads > 0x7fffffff ||
-        (int64_t(s->columns) << shift) > (1 << 30))
+        (int64_t(s->columns) << shift) > (1 << 30) || ((int64_t(s->columns) << shift) / 64 + 1) * s->heads > 0x7fffffff)
         return DLRB200_ERR_UNSUPPORTED_SHAPE;
     if (s->requests == 0) return DLRB200_OK;
     // (an empty cache, or a table without columns, holds no tokens)

@@ -37,13 +37,13 @@ constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
 // CTAs of an SM for heads of `dim`, nt groups of eight sharing keys: as many as registers and shared memory allow.  More warps
 // count for more than more copies in flight: a warp's step is a chain of dependent instructions (460 MB, us: 6 heads of 128 with
 // 3 CTAs of 3 or 4 halves 77, 2 CTAs of 5 or 6 halves 80; 3 heads of 256 with 2 CTAs of 2 halves 76, of 3 halves 80, one CTA of 4 85).
-constexpr int ctas_per_sm(int dim, int nt) { return dim == 64 ? (nt == 1 ? 5 : 4) : dim == 96 ? (nt == 1 ? 4 : 3) : dim == 128 ? 3 : 2; }
-constexpr int kMostCtasPerSm = 5;
-// Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (us):
-// 64 ragged requests of up to 8000 tokens, 8 heads of 128: 178 / 174 / 169 / 168; 200 of up to 1500, 12 heads of 64: 91 / 89
-// / 87 / 86; one of 131072, 8 heads: 93 / 92 / 95 / 98 where runs are 14 tiles and 9, 92 where they stay above 16.
+constexpr int ctas_per_sm(int dim, int nt) { return dim == 64 ? 4 : dim == 96 ? (nt == 1 ? 4 : 3) : dim == 128 ? 3 : 2; }
+constexpr int kMostCtasPerSm = 4;
+// Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (kernel and
+// join, us): 64 ragged requests of up to 8000 tokens, 8 heads of 128: 173 / 168 / 164 / 164; one of 131072: 93 / 92 / 92 / 94; 200
+// of up to 1500, 12 heads of 64: 83 / 84 / 83 / 90 with at least 32 / 8 / 32 / 8 tiles.
 constexpr int kWaves = 4;
-constexpr int kLeastRun = 16;
+constexpr int least_run(int dim) { return dim == 64 ? 32 : 16; }
 constexpr int kMostSms = 160;
 constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -57,8 +57,12 @@ struct Shape {
     static constexpr int kRows = 8 * NT;                           // query heads of a segment
     static constexpr int kJoinRow = D + 4;                         // floats; the padding keeps banks apart
     static constexpr int kJoin = kWarpsA * kRows * kJoinRow * 4;   // output of every warp; its maxima and sums lie behind
-    static constexpr int kSmem = (kRing > kJoin ? kRing : kJoin) + kWarpsA * kRows * 8;
     static constexpr int kCtasPerSm = ctas_per_sm(D, NT);
+    // the join has memory of its own where there is room, so that the next segment's copies can start before it
+    static constexpr int kMl = kWarpsA * kRows * 8;
+    static constexpr bool kApart = kRing + kJoin + kMl + 1280 <= 228 * 1024 / kCtasPerSm;
+    static constexpr int kJoinAt = kApart ? kRing : 0, kMlAt = kApart ? kRing + kJoin : kRing > kJoin ? kRing : kJoin;
+    static constexpr int kSmem = kMlAt + kMl;
     static constexpr int kPart = kRows * (D + 2);                  // floats of a partial result: output, maxima, sums
 };
 
@@ -227,92 +231,108 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
     before = place.before;
 
     const uint32_t ring = smem_u32(smem) + warp * (S::kHalves * S::kHalf);
-    float* const join = reinterpret_cast<float*>(smem);
-    float2* const join_ml = reinterpret_cast<float2*>(smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin));
+    float* const join = reinterpret_cast<float*>(smem + S::kJoinAt);
+    float2* const join_ml = reinterpret_cast<float2*>(smem + S::kMlAt);
     const float scale = p.scale * kLog2e;
     const uint64_t hint = l2_policy_evict_first();
 
-    for (; at < end;) {
-        // the segment that holds tile `at`
-        const int tokens = geo.tokens(request);
-        const int seg_tiles = (tokens + kTile - 1) / kTile;
-        if (at >= before + (long long)seg_tiles * geo.segments) {
-            before += (long long)seg_tiles * geo.segments;
-            ++request;
-            continue;
-        }
-        const int segment = int((at - before) / seg_tiles);
-        const int tile0 = int(at - before - (long long)segment * seg_tiles);
-        const long long left = end - at;
-        const int tile1 = seg_tiles - tile0 < left ? seg_tiles : tile0 + int(left);
-        const int kv_head = segment / groups, group = segment - kv_head * groups;
-        const int head0 = kv_head * group_size + group * S::kRows;
-        const int rows = min(S::kRows, group_size - group * S::kRows);
-        const int* const table = p.block_table + request * p.table_stride;
-        const T* const k_head = static_cast<const T*>(p.k_cache) + kv_head * p.k_head;
-        const T* const v_head = static_cast<const T*>(p.v_cache) + kv_head * p.v_head;
-
-        // this warp's steps: unit u covers the 16 tokens from u * 16, u = first, first + 4, ...
-        const int first = tile0 * kWarpsA + warp;
-        const int units = min(tile1 * kWarpsA, (tokens + kUnit - 1) / kUnit);
-        const int steps = first < units ? (units - first + kWarpsA - 1) / kWarpsA : 0;
-
-        // pages of the steps to come: lane i holds that of step 32 * n + i
-        int page_ids = 0;
-        auto load_pages = [&](int step) {
-            const int s = step + lane;
-            int id = -1;
-            if (s < steps) id = table[((first + s * kWarpsA) * kUnit) >> p.page_shift];
-            page_ids = id;
-        };
-        // copies half n of the steps: the keys of step n / 2, or its values
-        int in = 0;
-        auto fetch = [&](int n) {
-            const int step = n >> 1;
-            if (step < steps) {
-                if ((n & 63) == 0) load_pages(step);
-                const int page = __shfl_sync(~0u, page_ids, step & 31);
-                const int token0 = (first + step * kWarpsA) * kUnit;
-                const int slot0 = token0 & ((1 << p.page_shift) - 1);
-                const int valid = unsigned(page) < unsigned(p.pages) ? min(kUnit, tokens - token0) : 0;
-                const T* const src = (n & 1 ? v_head + (valid ? page : 0) * p.v_page : k_head + (valid ? page : 0) * p.k_page);
-                const int64_t slot_stride = n & 1 ? p.v_slot : p.k_slot;
-                const uint32_t stage = ring + in * S::kHalf;
-                constexpr int kChunks = D / 8;
-#pragma unroll
-                for (int i = 0; i < kUnit * kChunks / 32; ++i) {
-                    const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
-                    const uint32_t bytes = row < valid ? 16 : 0;
-                    const int slot = row < valid ? slot0 + row : 0;
-                    cp_async16(stage + row * S::kRow + col * 16, src + slot * slot_stride + col * 8, bytes, hint);
-                }
+    // The run's next segment, as far as it lies in the run; none: 0 tokens.
+    struct Piece {
+        int request, tokens, segment, tile0, tile1, seg_tiles;
+        bool opens;                             // it is the run's first
+    };
+    auto next_piece = [&]() {
+        Piece a{};
+        while (at < end) {
+            a.tokens = geo.tokens(request);
+            a.seg_tiles = (a.tokens + kTile - 1) / kTile;
+            const long long behind = before + (long long)a.seg_tiles * geo.segments;
+            if (at < behind) {
+                a.request = request;
+                a.segment = int(unsigned(at - before) / unsigned(a.seg_tiles));      // (below 2^31: host check)
+                a.tile0 = int(at - before) - a.segment * a.seg_tiles;
+                const long long left = end - at;
+                a.tile1 = a.seg_tiles - a.tile0 < left ? a.seg_tiles : a.tile0 + int(left);
+                a.opens = at == run * blockIdx.x;
+                at += a.tile1 - a.tile0;
+                return a;
             }
-            cp_async_commit();
-            in = in + 1 == S::kHalves ? 0 : in + 1;
-        };
+            before = behind;
+            ++request;
+        }
+        a.tokens = 0;
+        return a;
+    };
+
+    // The copies.  Of a piece, this warp takes the 16 tokens from u * 16, u = first, first + 4, ...: `steps` of them.
+    int tokens, first, steps, page_ids, in = 0, at_half = 0;
+    const int* table;
+    const T *k_head, *v_head;
+    // copies half n of the steps: the keys of step n / 2, or its values
+    auto fetch = [&](int n) {
+        const int step = n >> 1;
+        if (step < steps) {
+            if ((n & 63) == 0) {                // pages of the steps to come: lane i holds that of step 32 * k + i
+                const int s = step + lane;
+                page_ids = s < steps ? table[((first + s * kWarpsA) * kUnit) >> p.page_shift] : -1;
+            }
+            const int page = __shfl_sync(~0u, page_ids, step & 31);
+            const int token0 = (first + step * kWarpsA) * kUnit;
+            const int slot0 = token0 & ((1 << p.page_shift) - 1);
+            const int valid = unsigned(page) < unsigned(p.pages) ? min(kUnit, tokens - token0) : 0;
+            const T* const src = (n & 1 ? v_head + (valid ? page : 0) * p.v_page : k_head + (valid ? page : 0) * p.k_page);
+            const int64_t slot_stride = n & 1 ? p.v_slot : p.k_slot;
+            const uint32_t stage = ring + in * S::kHalf;
+            constexpr int kChunks = D / 8;
+#pragma unroll
+            for (int i = 0; i < kUnit * kChunks / 32; ++i) {
+                const int c = i * 32 + lane, row = c / kChunks, col = c % kChunks;
+                const uint32_t bytes = row < valid ? 16 : 0;
+                const int slot = row < valid ? slot0 + row : 0;
+                cp_async16(stage + row * S::kRow + col * 16, src + slot * slot_stride + col * 8, bytes, hint);
+            }
+        }
+        cp_async_commit();
+        in = in + 1 == S::kHalves ? 0 : in + 1;
+    };
+    // queries: row lane / 4 (and + 8), as the first operand of the products with 16 values each
+    uint32_t q[D / 16][2 * NT];
+    int head0, rows;
+    auto begin_piece = [&](const Piece& a) {
+        const int kv_head = a.segment / groups, group = a.segment - kv_head * groups;
+        tokens = a.tokens;
+        first = a.tile0 * kWarpsA + warp;
+        const int units = min(a.tile1 * kWarpsA, (tokens + kUnit - 1) / kUnit);
+        steps = first < units ? (units - first + kWarpsA - 1) / kWarpsA : 0;
+        table = p.block_table + a.request * p.table_stride;
+        k_head = static_cast<const T*>(p.k_cache) + kv_head * p.k_head;
+        v_head = static_cast<const T*>(p.v_cache) + kv_head * p.v_head;
+        in = at_half;                           // (the ring is empty)
 #pragma unroll
         for (int n = 0; n < S::kHalves - 1; ++n) fetch(n);
-
-        // queries: row lane / 4 (and + 8), as the first operand of the products with 16 values each
-        uint32_t q[D / 16][2 * NT];
-        {
-            const uint32_t* row[2];
-            bool on[2];
+        head0 = kv_head * group_size + group * S::kRows;
+        rows = min(S::kRows, group_size - group * S::kRows);
+        const uint32_t* row[2];
+        bool on[2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int h = lane / 4 + 8 * n;
+            on[n] = h < rows;
+            row[n] = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + a.request * p.q_request + (head0 + (on[n] ? h : 0)) * p.q_head) + lane % 4;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int h = lane / 4 + 8 * n;
-                on[n] = h < rows;
-                row[n] = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + request * p.q_request + (head0 + (on[n] ? h : 0)) * p.q_head) + lane % 4;
+                q[k][n] = on[n] ? row[n][k * 8] : 0u;
+                q[k][NT + n] = on[n] ? row[n][k * 8 + 4] : 0u;
             }
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    q[k][n] = on[n] ? row[n][k * 8] : 0u;
-                    q[k][NT + n] = on[n] ? row[n][k * 8 + 4] : 0u;
-                }
-        }
+    };
 
+    Piece piece = next_piece();
+    begin_piece(piece);
+    while (true) {
+        const Piece next = next_piece();
         // output, turned round: 16 values of a head times 8 heads to a tile
         float o[NT][D / 16][4], m[NT], l[NT];
 #pragma unroll
@@ -327,7 +347,6 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
 
         // both products take 8 x 8 blocks of a stage in the same order: tokens 0-7 and 8-15, of each two runs of eight values
         const uint32_t in_stage = ((lane & 7) + ((lane >> 4) & 1) * 8) * S::kRow + ((lane >> 3) & 1) * 16;
-        int at_half = 0;
         auto next_half = [&](int n) {
             cp_async_wait<S::kHalves - 2>();
             __syncwarp();                       // the half's copies are there, and every lane is done with the one before
@@ -410,8 +429,13 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, lo[n][0], lo[n][1]);
             }
         }
-        cp_async_wait<0>();
-        __syncthreads();                        // the rings are free
+        const int out_head = head0, out_rows = rows;
+        if constexpr (S::kApart) {
+            if (next.tokens) begin_piece(next);
+        } else {
+            cp_async_wait<0>();
+            __syncthreads();                    // the rings are free
+        }
 
         // the warps' results: maxima and sums, outputs
 #pragma unroll
@@ -429,9 +453,9 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
         }
         __syncthreads();
         // (more than one CTA: the rest is joined by join_kernel)
-        const bool whole = tile0 == 0 && tile1 == seg_tiles;
-        float* const part = static_cast<float*>(p.workspace) + (int64_t(blockIdx.x) * 2 + (at == run * blockIdx.x ? 0 : 1)) * S::kPart;
-        for (int i = threadIdx.x; i < rows * (D / 2); i += kThreadsA) {
+        const bool whole = piece.tile0 == 0 && piece.tile1 == piece.seg_tiles;
+        float* const part = static_cast<float*>(p.workspace) + (int64_t(blockIdx.x) * 2 + (piece.opens ? 0 : 1)) * S::kPart;
+        for (int i = threadIdx.x; i < out_rows * (D / 2); i += kThreadsA) {
             const int row = i / (D / 2), c = (i % (D / 2)) * 2;
             float2 ml[kWarpsA];
             float top = -INFINITY;
@@ -453,15 +477,18 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
             }
             if (whole) {
                 const float inv = 1.f / sum;
-                *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(request) * p.heads + head0 + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(piece.request) * p.heads + out_head + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
             } else {
                 *reinterpret_cast<float2*>(part + row * D + c) = v;
                 if (c == 0) *reinterpret_cast<float2*>(part + S::kRows * D + row * 2) = make_float2(top, sum);
             }
         }
-        __syncthreads();                        // the rings are written again
-        at += tile1 - tile0;
+        if (!next.tokens) break;
+        __syncthreads();                        // the join's memory is written again
+        if constexpr (!S::kApart) begin_piece(next);
+        piece = next;
     }
+    cp_async_wait<0>();
 }
 
 // Where a head's partial results are: `parts` of them, in the slots of runs `run`, run + 1, ...
@@ -631,7 +658,7 @@ cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
     const int group_size = a.heads / a.kv_heads, groups = (group_size + S::kRows - 1) / S::kRows;
     // no more CTAs than the table could hold tiles
     const long long most = (long long)a.requests * a.kv_heads * groups * (((long long)a.columns << a.page_shift) / kTile + 1);
-    Cut cut{S::kCtasPerSm * min(num_sms, kMostSms), kWaves, kLeastRun};
+    Cut cut{S::kCtasPerSm * min(num_sms, kMostSms), kWaves, least_run(D)};
     if (most < cut.resident) cut.resident = int(most);
     const int ctas = cut.resident * kWaves;
     kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups, cut);
