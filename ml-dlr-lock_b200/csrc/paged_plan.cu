@@ -77,6 +77,7 @@ __device__ __forceinline__ int owner(const int* first, int n, int a) {
 template <bool CLUSTER>
 __device__ __forceinline__ void barrier() {
     if constexpr (CLUSTER) {
+        __syncwarp();                        // (the barrier is one of whole warps)
         cluster_arrive_release();
         cluster_wait_acquire();
     } else {

@@ -259,6 +259,66 @@ def test_gradients_of_part_of_the_outputs_and_repeats():
     assert out[0].shape == (3, 100, 16, 128)
 
 
+def test_norm_rope_of_no_tokens_of_layouts_that_are_copied_and_twice():
+    import dlr_lock_b200 as D
+    q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(24, 4, 2, 64, 32, torch.float16, True, True)
+    # no tokens: empty outputs, gradients of zero
+    leaves = [t.detach().requires_grad_(True) for t in (q[:0], k[:0], qw, kw)]
+    out = D.qk_norm_rope(*leaves, cos, sin, positions[:0])
+    got = torch.autograd.grad(out, leaves, [torch.zeros_like(o) for o in out])
+    assert [tuple(o.shape) for o in out] == [(0, 4, 64), (0, 2, 64)] and not got[2].any() and not got[3].any()
+    cache = torch.zeros(1, 2, 16, 64, dtype=torch.float16, device=DEV)
+    assert D.qk_norm_rope_append(q[:0], k[:0], v[:0], qw, kw, cos, sin, positions[:0], positions[:0].int(), cache, cache.clone()).shape == (0, 4, 64)
+    # what cannot be read where it lies gives the same bits: other orders, a weight and rows off their boundaries
+    want = D.qk_norm_rope(q, k, qw, kw, cos, sin, positions, interleaved=True)
+    off = torch.empty(65, dtype=torch.float16, device=DEV)[1:].copy_(qw)
+    wide = torch.empty(24, 4 * 64 + 1, dtype=torch.float16, device=DEV)
+    wide[:, 1:] = q.flatten(1)
+    for q2, w2 in ((q.transpose(0, 1).contiguous().transpose(0, 1), qw), (q.transpose(1, 2).contiguous().transpose(1, 2), off),
+                   (wide[:, 1:].unflatten(-1, (4, 64)), qw)):
+        got = D.qk_norm_rope(q2, k, w2, kw, cos, sin, positions, interleaved=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    batched = q.view(4, 6, 4, 64).transpose(0, 1), k.view(4, 6, 2, 64).transpose(0, 1), positions.view(4, 6).t()      # (6, 4, ...)
+    leaf = batched[0].detach().requires_grad_(True)
+    got = D.qk_norm_rope(leaf, batched[1], qw, kw, cos, sin, batched[2], interleaved=True)
+    assert torch.equal(got[0], want[0].view(4, 6, 4, 64).transpose(0, 1))
+    g = torch.autograd.grad(got[0].float().sum(), leaf)[0]
+    straight = q.detach().requires_grad_(True)
+    assert torch.equal(g, torch.autograd.grad(D.qk_norm_rope(straight, k, qw, kw, cos, sin, positions, interleaved=True)[0].float().sum(),
+                                              straight)[0].view(4, 6, 4, 64).transpose(0, 1))
+    # a gradient of the gradient is refused, not taken for zero
+    leaf = q.detach().requires_grad_(True)
+    once = torch.autograd.grad(D.qk_norm_rope(leaf, k, qw, kw, cos, sin, positions)[0].float().square().sum(), leaf, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(once.float().sum(), leaf)
+
+
+def test_norm_rope_gradient_captured():
+    import dlr_lock_b200 as D
+    q, k, _, qw, kw, cos, sin, positions = _norm_rope_case(200, 8, 2, 128, 64, torch.bfloat16, False, True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    gen = _gen(9)
+    grads = [_normal(gen, *t.shape, dtype=t.dtype) for t in (q, k)]
+
+    def step():
+        out = D.qk_norm_rope(*leaves, cos, sin, positions)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, leaves, grads))
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_norm_rope_positions_outside_the_tables_give_nan_rows():
     import dlr_lock_b200 as D
     q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(6, 4, 2, 64, 16, torch.float16, False, True)
@@ -409,6 +469,38 @@ def test_attention_orders_and_strides():
     q = wide[:, 1:1 + 6 * 64].unflatten(-1, (6, 64))
     got = D.paged_attention(q, kc, vc, table, torch.tensor(lengths, dtype=torch.int32, device=DEV))
     _close(got, *_attend64(q, kc, vc, table, lengths, 0.125))
+
+
+def test_attention_of_no_requests_no_columns_no_pages():
+    import dlr_lock_b200 as D
+    kc, vc, table, n = _cache_case([70, 5], 2, 64, 32, torch.bfloat16)
+    q = _normal(_gen(1), 2, 4, 64, dtype=torch.bfloat16)
+    assert D.paged_attention(q[:0], kc, vc, table[:0], n[:0]).shape == (0, 4, 64)
+    assert not D.paged_attention(q, kc, vc, table[:, :0], n).any()
+    assert not D.paged_attention(q, kc[:0], vc[:0], table, n).any()
+
+
+def test_attention_with_offsets_beyond_32_bits():
+    # keys and values of 2^32 elements each, the values behind the keys
+    import dlr_lock_b200 as D
+    whole = torch.empty(2, 2 ** 22, 1, 16, 64, dtype=torch.float16, device=DEV)
+    kc, vc = whole[0], whole[1]
+    gen = _gen(3)
+    q = _normal(gen, 1, 2, 64, dtype=torch.float16)
+    ids = [2 ** 22 - 1, 0, 2 ** 22 - 2, 2 ** 21 + 1]
+    table = torch.tensor([ids], dtype=torch.int32, device=DEV)
+    for i in ids:
+        kc[i], vc[i] = (_normal(gen, 1, 16, 64, dtype=torch.float16) for _ in range(2))
+    got = D.paged_attention(q, kc, vc, table, torch.tensor([60], dtype=torch.int32, device=DEV))
+    _close(got, *_attend64(q, kc, vc, table, [60], 0.125))
+    row = _normal(gen, 1, 1, 64, dtype=torch.float16)
+    slot = (2 ** 22 - 1) * 16 + 15
+    cos, sin = D.rope_tables(torch.ones(32, device=DEV), 4)
+    D.qk_norm_rope_append(row, row, row, None, None, cos, sin, torch.zeros(1, dtype=torch.int32, device=DEV),
+                          torch.tensor([slot], dtype=torch.int32, device=DEV), kc, vc)
+    assert torch.equal(kc[2 ** 22 - 1, 0, 15], row[0, 0]) and torch.equal(vc[2 ** 22 - 1, 0, 15], row[0, 0])
+    del whole, kc, vc
+    torch.cuda.empty_cache()
 
 
 def test_attention_far_scores_and_hidden_tokens():
