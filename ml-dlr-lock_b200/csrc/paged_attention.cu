@@ -2,14 +2,15 @@
 //
 //   o_h = sum_j softmax_j(scale * q_h . k_j) v_j     over the tokens j of the request; zeros where there are none
 //
-// Bound by memory: the keys and values of a request are read once for all query heads that share them (64 bytes per
-// multiply-add of each of dim values and head: far below what the tensor cores give), and nothing else is big.
+// Bound by memory: the keys and values of a request are read once for all query heads that share them, and each value read serves
+// one multiply-add for each of these heads, far below what the tensor cores give.
 //
 // Split.  The work is a list of tiles of 64 tokens: request by request, key-value head by key-value head.  It is cut into
-// equal runs, one per CTA, wherever the cuts fall: short requests share a CTA, a long one is spread over all of them, ragged
+// equal runs, a few for each CTA, wherever the cuts fall: short requests share a CTA, a long one is spread over all of them, ragged
 // batches stay balanced, and the host needs to know no length.  A CTA works through its run segment by segment (the tiles of
 // one request and head).  What is cut is joined by a second, small kernel from partial results in fp32, in the order of the
-// tokens, so that results repeat bit for bit; what is whole is finished by its CTA.
+// tokens, so that results repeat bit for bit; what is whole is finished by its CTA.  Where the table holds short contexts only, a
+// cluster takes each head's tokens instead and joins them through distributed shared memory: one launch.
 //
 // A warp takes 16 tokens of a tile at a time, on its own: it copies their keys and their values to its own ring in shared memory
 // (cp.async, rows padded by 16 bytes so that ldmatrix meets no bank twice), multiplies with mma.sync, and keeps maximum, sum and
@@ -44,6 +45,12 @@ constexpr int kMostCtasPerSm = 4;
 // of up to 1500, 12 heads of 64: 83 / 84 / 83 / 90 with at least 32 / 8 / 32 / 8 tiles.
 constexpr int kWaves = 4;
 constexpr int least_run(int dim) { return dim == 64 ? 32 : 16; }
+constexpr int kMostShares = 8;                   // CTAs of a cluster
+// Tiles of a share up to which a cluster for each segment is taken instead of the runs and their join, by what the table could
+// hold (the host knows no lengths).  us, runs / clusters, contexts of one length, then ragged ones: 1 request of 513 tokens, 8
+// heads of 128, 2 tiles: 5.7 / 4.7; 8 of 768, 2 tiles: 9.7 / 7.1, 8.7 / 6.8; 8 of 2000, 8 tiles: 15.6 / 11.7, 12.5 / 10.5; 32 of
+// 768, 12 tiles: 20.9 / 16.2, 15.0 / 13.4; 256 of 700, 11 tiles: 135 / 119, 69 / 63.  Above: 64 of 1000, 16 tiles: 51 / 57, 34 / 31.
+constexpr int kShort = 12;
 constexpr int kMostSms = 160;
 constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -120,6 +127,12 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     }
 }
 
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr_cluster) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr_cluster) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(~0u, v, 1));
     return fmaxf(v, __shfl_xor_sync(~0u, v, 2));
@@ -183,52 +196,58 @@ struct Place {
     long long before;
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut) {
+// SHARED: a cluster of `shares` CTAs to each segment instead, which take equal shares of its tiles and are joined through
+// distributed shared memory (short contexts, where a second launch would cost as much as the work).
+template <typename T, int D, int NT, bool SHARED>
+__global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_attention_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut, int shares) {
     using S = Shape<D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ long long scratch[kWarpsA];
     __shared__ Place place;
+    __shared__ float2 share_ml[S::kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int group_size = p.heads / p.kv_heads;
     const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
 
-    asm volatile("griddepcontrol.launch_dependents;");
-
-    // all tiles, and the request in which this CTA's run begins
-    long long total = 0, mine = 0, before = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
-        const int r = r0 + int(threadIdx.x);
-        long long here;
-        mine = r < p.requests ? geo.tiles(r) : 0;
-        before = total + scan_tiles<kWarpsA>(mine, scratch, &here);
-        total += here;
-    }
-    const long long run = cut.run(total);
-    long long at = run * blockIdx.x;
-    const long long end = at + run < total ? at + run : total;
-    // requests without tokens belong to no tile: their zeros are written by the CTAs in turn
-    for (int r = blockIdx.x; r < p.requests; r += gridDim.x)
-        if (geo.tokens(r) == 0)
-            for (int i = threadIdx.x; i < p.heads * D / 2; i += kThreadsA)
-                reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + int64_t(r) * p.heads * D)[i] = 0;
-    if (at >= end) return;
-    if (p.requests <= kThreadsA) {
-        if (at >= before && at < before + mine) place = {int(threadIdx.x), before};
-    } else {
-        long long base = 0;
+    long long run = 0, at = 0, end = 0, before = 0;
+    int request = 0;
+    if constexpr (!SHARED) {
+        asm volatile("griddepcontrol.launch_dependents;");
+        // all tiles, and the request in which this CTA's run begins
+        long long total = 0, mine = 0;
         for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
             const int r = r0 + int(threadIdx.x);
-            mine = r < p.requests ? geo.tiles(r) : 0;
             long long here;
-            before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
-            if (at >= before && at < before + mine) place = {r, before};
-            base += here;
+            mine = r < p.requests ? geo.tiles(r) : 0;
+            before = total + scan_tiles<kWarpsA>(mine, scratch, &here);
+            total += here;
         }
+        run = cut.run(total);
+        at = run * blockIdx.x;
+        end = at + run < total ? at + run : total;
+        // requests without tokens belong to no tile: their zeros are written by the CTAs in turn
+        for (int r = blockIdx.x; r < p.requests; r += gridDim.x)
+            if (geo.tokens(r) == 0)
+                for (int i = threadIdx.x; i < p.heads * D / 2; i += kThreadsA)
+                    reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + int64_t(r) * p.heads * D)[i] = 0;
+        if (at >= end) return;
+        if (p.requests <= kThreadsA) {
+            if (at >= before && at < before + mine) place = {int(threadIdx.x), before};
+        } else {
+            long long base = 0;
+            for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
+                const int r = r0 + int(threadIdx.x);
+                mine = r < p.requests ? geo.tiles(r) : 0;
+                long long here;
+                before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
+                if (at >= before && at < before + mine) place = {r, before};
+                base += here;
+            }
+        }
+        __syncthreads();
+        request = place.request;
+        before = place.before;
     }
-    __syncthreads();
-    int request = place.request;
-    before = place.before;
 
     const uint32_t ring = smem_u32(smem) + warp * (S::kHalves * S::kHalf);
     float* const join = reinterpret_cast<float*>(smem + S::kJoinAt);
@@ -329,10 +348,24 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
             }
     };
 
-    Piece piece = next_piece();
+    Piece piece;
+    if constexpr (SHARED) {
+        const int mine = int(blockIdx.x) / shares, rank = int(blockIdx.x) - mine * shares;
+        piece.request = mine / geo.segments;
+        piece.segment = mine - piece.request * geo.segments;
+        piece.tokens = geo.tokens(piece.request);
+        piece.seg_tiles = (piece.tokens + kTile - 1) / kTile;
+        const int each = (piece.seg_tiles + shares - 1) / shares;
+        piece.tile0 = min(rank * each, piece.seg_tiles);
+        piece.tile1 = min(piece.tile0 + each, piece.seg_tiles);
+        piece.opens = true;
+    } else {
+        piece = next_piece();
+    }
     begin_piece(piece);
     while (true) {
-        const Piece next = next_piece();
+        Piece next{};
+        if constexpr (!SHARED) next = next_piece();
         // output, turned round: 16 values of a head times 8 heads to a tile
         float o[NT][D / 16][4], m[NT], l[NT];
 #pragma unroll
@@ -475,13 +508,49 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 v.x += f * x.x;
                 v.y += f * x.y;
             }
-            if (whole) {
+            if constexpr (SHARED) {             // kept where warp 0's was, for the cluster
+                *reinterpret_cast<float2*>(join + row * S::kJoinRow + c) = v;
+                if (c == 0) share_ml[row] = make_float2(top, sum);
+            } else if (whole) {
                 const float inv = 1.f / sum;
                 *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(piece.request) * p.heads + out_head + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
             } else {
                 *reinterpret_cast<float2*>(part + row * D + c) = v;
                 if (c == 0) *reinterpret_cast<float2*>(part + S::kRows * D + row * 2) = make_float2(top, sum);
             }
+        }
+        if constexpr (SHARED) {
+            __syncthreads();
+            cluster_arrive_release();
+            cluster_wait_acquire();             // every share's result is in its CTA's shared memory
+            const int rank = int(cluster_ctarank());
+            for (int i = rank * kThreadsA + int(threadIdx.x); i < out_rows * (D / 2); i += shares * kThreadsA) {
+                const int row = i / (D / 2), c = (i % (D / 2)) * 2;
+                const uint32_t at_v = smem_u32(join + row * S::kJoinRow + c), at_ml = smem_u32(&share_ml[row]);
+                float2 ml[kMostShares], x[kMostShares];
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kMostShares; ++w) {
+                    ml[w] = w < shares ? ld_cluster_f2(mapa(at_ml, w)) : make_float2(-INFINITY, 0.f);
+                    x[w] = w < shares ? ld_cluster_f2(mapa(at_v, w)) : make_float2(0.f, 0.f);
+                    top = fmaxf(top, ml[w].x);
+                }
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = 0.f;
+                float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kMostShares; ++w) {
+                    const float f = exp2f(ml[w].x - ref);
+                    sum += f * ml[w].y;
+                    v.x += f * x[w].x;
+                    v.y += f * x[w].y;
+                }
+                const float inv = piece.tokens ? 1.f / sum : 0.f;        // (no tokens: zeros)
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(piece.request) * p.heads + out_head + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
+            }
+            __syncwarp();
+            cluster_arrive_release();
+            cluster_wait_acquire();             // nobody reads this CTA's shared memory any more
         }
         if (!next.tokens) break;
         __syncthreads();                        // the join's memory is written again
@@ -499,7 +568,7 @@ struct Pieces {
 // Joins the runs over which segments were cut: `per_cta` (1 or 8) query heads to a CTA.  It is launched while the first kernel
 // still runs and finds its place in the work meanwhile.  A warp joins a head of few parts by itself, all warps of the CTA one of
 // many; maxima come first, so that the loads of the parts do not wait for one another.  Sums run in the order of the tokens.
-// (Measured behind the first kernel, us: 6 for 64 heads of 108 parts each.)
+// (Behind the first kernel it takes 3 us.)
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut, int per_cta) {
     using S = Shape<D, NT>;
@@ -652,16 +721,36 @@ __global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__
 template <typename T, int D, int NT>
 cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
     using S = Shape<D, NT>;
-    auto kern = paged_attention_kernel<T, D, NT>;
+    const int group_size = a.heads / a.kv_heads, groups = (group_size + S::kRows - 1) / S::kRows;
+    const long long segments = (long long)a.requests * a.kv_heads * groups, resident = S::kCtasPerSm * min(num_sms, kMostSms);
+    // what the table could hold, in tiles of a segment
+    const long long tiles = (((long long)a.columns << a.page_shift) + kTile - 1) / kTile;
+    int shares = 1;
+    while (shares < kMostShares && shares < tiles && segments * shares * 2 <= resident) shares *= 2;
+    if (tiles <= kShort * shares && segments * shares <= 0x7fffffff) {
+        auto kern = paged_attention_kernel<T, D, NT, true>;
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return e;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim = {unsigned(shares), 1, 1};
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(segments * shares));
+        cfg.blockDim = dim3(kThreadsA);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.stream = stream;
+        cfg.attrs = &cluster;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kern, a, groups, Cut{}, shares);
+    }
+    auto kern = paged_attention_kernel<T, D, NT, false>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
-    const int group_size = a.heads / a.kv_heads, groups = (group_size + S::kRows - 1) / S::kRows;
     // no more CTAs than the table could hold tiles
-    const long long most = (long long)a.requests * a.kv_heads * groups * (((long long)a.columns << a.page_shift) / kTile + 1);
-    Cut cut{S::kCtasPerSm * min(num_sms, kMostSms), kWaves, least_run(D)};
-    if (most < cut.resident) cut.resident = int(most);
-    const int ctas = cut.resident * kWaves;
-    kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups, cut);
+    const long long most = segments * tiles < 1 ? 1 : segments * tiles;
+    const Cut cut{int(most < resident ? most : resident), kWaves, least_run(D)};
+    const int ctas = int(most < (long long)cut.resident * kWaves ? most : (long long)cut.resident * kWaves);
+    kern<<<ctas, kThreadsA, S::kSmem, stream>>>(a, groups, cut, 1);
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;

@@ -423,8 +423,12 @@ def _check_attention(lengths, heads, kv_heads, dim, page, dtype, scale=None, **k
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (16, 8), (12, 12), (5, 1), (32, 4), (27, 3), (16, 1), (40, 2), (17, 1)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_attention_heads(dim, heads, kv_heads, dtype):
-    # lengths around the step of 16 tokens, the tile of 64 and the page, none among them
-    _check_attention([1, 0, 15, 16, 17, 63, 64, 65, 200, 0], heads, kv_heads, dim, 32, dtype)
+    # lengths around the step of 16 tokens, the tile of 64 and the page, none among them; a table of short contexts (clusters) and
+    # one with room for long ones (runs and their join), which give the same up to the order of sums
+    lengths = [1, 0, 15, 16, 17, 63, 64, 65, 200, 0]
+    _check_attention(lengths, heads, kv_heads, dim, 32, dtype)
+    _check_attention(lengths, heads, kv_heads, dim, 32, dtype, columns=1000)
+    _check_attention([4000, 0, 700], heads, kv_heads, dim, 32, dtype, columns=1000)
 
 
 @pytest.mark.parametrize("page", [16, 32, 128, 1024])
@@ -434,16 +438,18 @@ def test_attention_lengths(page, lengths):
     _check_attention(lengths, 8, 2, 128, page, "bf16", seed=len(lengths) + page)
 
 
+@pytest.mark.parametrize("columns", [None, 900])
 @pytest.mark.parametrize("requests", [129, 300])
-def test_attention_many_requests(requests):
+def test_attention_many_requests(requests, columns):
     rng = random.Random(requests)
-    _check_attention([rng.choice([0, 1, rng.randint(0, 700)]) for _ in range(requests)], 6, 2, 64, 16, "fp16")
+    _check_attention([rng.choice([0, 1, rng.randint(0, 700)]) for _ in range(requests)], 6, 2, 64, 16, "fp16", columns=columns)
 
 
+@pytest.mark.parametrize("columns", [9, 900])
 @pytest.mark.parametrize("fill", [float("nan"), float("inf"), -65504.0])
-def test_attention_never_reads_what_no_request_holds(fill):
+def test_attention_never_reads_what_no_request_holds(fill, columns):
     # the rest of a page, pages of nobody, and table entries beyond the length (outside the cache)
-    _check_attention([1, 15, 33, 0, 129], 8, 4, 64, 32, "fp16", fill=fill, columns=9)
+    _check_attention([1, 15, 33, 0, 129], 8, 4, 64, 32, "fp16", fill=fill, columns=columns)
 
 
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3, 3.0])
@@ -536,9 +542,10 @@ def test_attention_table_entries_outside_the_cache_count_as_zeros():
 
 
 # ---- streams, graphs, and all of it together --------------------------------------------------------------------------------
-def test_attention_on_another_stream_and_replayed_with_other_lengths():
+@pytest.mark.parametrize("columns", [None, 500])
+def test_attention_on_another_stream_and_replayed_with_other_lengths(columns):
     import dlr_lock_b200 as D
-    kc, vc, table, n = _cache_case([900, 40, 2000], 4, 128, 64, torch.bfloat16)
+    kc, vc, table, n = _cache_case([900, 40, 2000], 4, 128, 64, torch.bfloat16, columns=columns)
     q = _normal(_gen(2), 3, 16, 128, dtype=torch.bfloat16)
     want = D.paged_attention(q, kc, vc, table, n)
     side = torch.cuda.Stream()
@@ -567,12 +574,13 @@ def test_attention_on_another_stream_and_replayed_with_other_lengths():
     assert torch.equal(pair[0][2], want) and torch.equal(pair[1][2], want_other)
 
 
-def test_decode_steps_together_captured():
+@pytest.mark.parametrize("columns", [8, 1000])
+def test_decode_steps_together_captured(columns):
     """Plan, norm and rotation with append, attention: prompts admitted, then steps replayed from one graph, against the same
     attention over everything that a request was given."""
     import dlr_lock_b200 as D
     gen = _gen(11)
-    requests, heads, kv_heads, dim, page, columns = 5, 8, 2, 64, 16, 8
+    requests, heads, kv_heads, dim, page = 5, 8, 2, 64, 16
     dtype = torch.bfloat16
     kc, vc = (torch.full((30, kv_heads, page, dim), float("nan"), dtype=dtype, device=DEV) for _ in range(2))
     table = torch.full((requests, columns), -1, dtype=torch.int32, device=DEV)
