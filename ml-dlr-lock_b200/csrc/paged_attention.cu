@@ -142,6 +142,8 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor_sync(~0u, v, 2);
 }
 
+constexpr int kEach = 8;                         // requests that a thread counts at a time
+
 // Tokens and tiles of a request.
 struct Geometry {
     const int* lengths;
@@ -152,7 +154,16 @@ struct Geometry {
         const long long n = lengths[r];
         return int(n < 0 ? 0 : n > capacity ? capacity : n);
     }
-    __device__ __forceinline__ long long tiles(int r) const { return (long long)((tokens(r) + kTile - 1) / kTile) * segments; }
+    // tiles of the requests r, r + 1, ... that a thread counts, and all of them (below 2^31 for each: host check)
+    __device__ __forceinline__ long long some(int r, int (&tiles)[kEach]) const {
+        long long sum = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            tiles[k] = r + k < requests ? (tokens(r + k) + kTile - 1) / kTile * segments : 0;
+            sum += tiles[k];
+        }
+        return sum;
+    }
 };
 
 // Sums of v over the warps' lanes: what lies before this thread, and all.
@@ -214,12 +225,11 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
     if constexpr (!SHARED) {
         asm volatile("griddepcontrol.launch_dependents;");
         // all tiles, and the request in which this CTA's run begins
-        long long total = 0, mine = 0;
-        for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
-            const int r = r0 + int(threadIdx.x);
+        long long total = 0;
+        int mine[kEach];
+        for (int r0 = 0; r0 < p.requests; r0 += kThreadsA * kEach) {
             long long here;
-            mine = r < p.requests ? geo.tiles(r) : 0;
-            before = total + scan_tiles<kWarpsA>(mine, scratch, &here);
+            before = total + scan_tiles<kWarpsA>(geo.some(r0 + int(threadIdx.x) * kEach, mine), scratch, &here);
             total += here;
         }
         run = cut.run(total);
@@ -231,16 +241,22 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 for (int i = threadIdx.x; i < p.heads * D / 2; i += kThreadsA)
                     reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + int64_t(r) * p.heads * D)[i] = 0;
         if (at >= end) return;
-        if (p.requests <= kThreadsA) {
-            if (at >= before && at < before + mine) place = {int(threadIdx.x), before};
+        auto find = [&](int r, long long before) {
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                if (at >= before && at < before + mine[k]) place = {r + k, before};
+                before += mine[k];
+            }
+        };
+        if (p.requests <= kThreadsA * kEach) {
+            find(int(threadIdx.x) * kEach, before);
         } else {
             long long base = 0;
-            for (int r0 = 0; r0 < p.requests; r0 += kThreadsA) {
-                const int r = r0 + int(threadIdx.x);
-                mine = r < p.requests ? geo.tiles(r) : 0;
+            for (int r0 = 0; r0 < p.requests; r0 += kThreadsA * kEach) {
+                const int r = r0 + int(threadIdx.x) * kEach;
                 long long here;
-                before = base + scan_tiles<kWarpsA>(mine, scratch, &here);
-                if (at >= before && at < before + mine) place = {r, before};
+                before = base + scan_tiles<kWarpsA>(geo.some(r, mine), scratch, &here);
+                find(r, before);
                 base += here;
             }
         }
@@ -585,11 +601,15 @@ __global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__
     const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
     const int first_request = first_head / p.heads;
     long long total = 0;
-    for (int r0 = 0; r0 < p.requests; r0 += kThreadsJ) {
-        const int r = r0 + int(threadIdx.x);
-        long long here;
-        const long long at = total + scan_tiles<kWarpsJ>(r < p.requests ? geo.tiles(r) : 0, scratch, &here);
-        if (r >= first_request && r < first_request + per_cta) before[r - first_request] = at;
+    for (int r0 = 0; r0 < p.requests; r0 += kThreadsJ * kEach) {
+        const int r = r0 + int(threadIdx.x) * kEach;
+        int tiles[kEach];
+        long long here, at = total + scan_tiles<kWarpsJ>(geo.some(r, tiles), scratch, &here);
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (r + k >= first_request && r + k < first_request + per_cta) before[r + k - first_request] = at;
+            at += tiles[k];
+        }
         total += here;
     }
     __syncthreads();

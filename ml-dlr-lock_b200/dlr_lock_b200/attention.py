@@ -92,8 +92,8 @@ def _int32(what, name, t, shape):
 def _page_size(what, page_size):
     if type(page_size) is not int:
         raise TypeError(f"{what}: the page size must be an int, not {type(page_size).__name__}")
-    if page_size < 16 or page_size & (page_size - 1):
-        raise ValueError(f"{what}: pages have 2^n tokens, 16 or more, not {page_size}")
+    if not 16 <= page_size <= 1 << 20 or page_size & (page_size - 1):
+        raise ValueError(f"{what}: pages have 2^n tokens, 16 to 2^20, not {page_size}")
 
 
 def _check_cache(what, k_cache, v_cache, dtype, kv_heads, dim, multiple):

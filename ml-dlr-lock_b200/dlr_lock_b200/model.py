@@ -341,8 +341,12 @@ def head_norms(attn):
 
 
 def attention_fusable(attn) -> bool:
-    """Whether an attention module is projections, norms over each head (or none) and a rotation, on full attention."""
-    if not all(hasattr(attn, n) for n in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "scaling", "layer_idx")):
+    """Whether an attention module is projections, norms over each head (or none) and a rotation in halves, on full attention:
+    those of the decoders that ``registry.MODEL_CONFIGS`` names.  (Others may order the rotation's pairs in another way, which
+    nothing about the module shows.)"""
+    if not all(hasattr(attn, n) for n in ("q_proj", "k_proj", "v_proj", "o_proj", "head_dim", "scaling", "layer_idx", "config")):
+        return False
+    if getattr(attn.config, "model_type", None) != "qwen3":
         return False
     if getattr(attn, "sliding_window", None) or hasattr(attn, "sinks"):
         return False
