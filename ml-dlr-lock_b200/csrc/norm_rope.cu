@@ -47,32 +47,15 @@ __device__ __forceinline__ uint32_t from_floats<__half>(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// two fp32 values in a register pair: one instruction for both
-using Pair = unsigned long long;
-__device__ __forceinline__ Pair pair(float lo, float hi) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 floats(Pair p) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
-    return r;
-}
-__device__ __forceinline__ Pair swapped(Pair p) {
-    const float2 f = floats(p);
-    return pair(f.y, f.x);
-}
-__device__ __forceinline__ Pair mul(Pair a, Pair b) {
-    Pair r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-    Pair r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
+// two fp32 values
+struct Pair {
+    float x, y;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) { return {lo, hi}; }
+__device__ __forceinline__ float2 floats(Pair p) { return make_float2(p.x, p.y); }
+__device__ __forceinline__ Pair swapped(Pair p) { return {p.y, p.x}; }
+__device__ __forceinline__ Pair mul(Pair a, Pair b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) { return {fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
 
 // A lane's run of RUN neighbouring values of a head, as it lies in memory and as fp32 pairs.
 template <int RUN>
@@ -136,7 +119,7 @@ __device__ __forceinline__ void coefficients(const float* c, const float* s, boo
 #pragma unroll
         for (int j = 0; j < RUN; ++j) {
             own[j] = pair(1.f, 1.f);
-            other[j] = 0;
+            other[j] = {};
         }
     } else if constexpr (INTERLEAVED) {                  // cosine j belongs to the pair (2j, 2j + 1) of the two runs in a row
 #pragma unroll
@@ -236,11 +219,11 @@ __device__ __forceinline__ float head_sum(float v) {
 
 // ---- the lanes' queues --------------------------------------------------------------------------------------------------
 // A warp walks over units of (token, group of up to U * 32 / LPH heads).  Its lanes copy what the next unit needs into a queue in
-// shared memory (cp.async) while they work on this one, so that loads are in flight all the time without registers for them.
-// What bounds it is instruction issue as much as memory (800 instructions for a unit of 4 KB): values lie in register pairs and
-// are handled two at a time, and what the heads of a unit share (angles times weights) is formed once.  5001 tokens, 64 + 8 heads
-// of 128 with values: 41 us of 31.6 at copy bandwidth; 8192 tokens, 32 + 8 heads: 34 us of 25.6, backward 50 of 38.4.  With loads
-// into registers, unit after unit, values one at a time: 46, 38 and 82.
+// shared memory (cp.async) while they work on this one, so that loads are in flight all the time without registers for them.  What
+// the heads of a unit share (angles times weights) is formed once.  5001 tokens, 64 + 8 heads of 128 with values: 39 us, of 31.6 at
+// copy bandwidth (a plain elementwise pass over as many bytes takes 33, and so does this loop without the arithmetic 39: what is
+// left is its pattern of loads and stores); 8192 tokens, 32 + 8 heads: 31 us of 25.6, backward 50 of 38.4.  With loads into
+// registers, unit after unit: 46, 38 and 82.  Arithmetic on register pairs written as such (f32x2) was slower: 41, 33 and 50.
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <int BYTES>
@@ -264,10 +247,10 @@ struct Stage {
 
 constexpr int kStagesN = 2;
 // Heads one behind the other in a unit, and blocks of an SM.  Measured for 5001 tokens, 64 + 8 heads of 128 with values, and 8192
-// tokens, 32 + 8 heads (us): 41 / 34 with units of 4 and 4 or 5 blocks, 51 / 44 with units of 2, 58 / 47 with 6 blocks (registers
-// spill) or units of 8, 49 / 40 with a queue of three units (fewer warps fit); backward 49 with units of 2 and a queue of two, 54
-// with three, 65 with units of 1.
-constexpr int kForwardUnit = 4, kForwardBlocksPerSm = 5, kBackwardUnit = 2;
+// tokens, 32 + 8 heads (us): 39 / 31 with units of 4 and 4 or 5 blocks, 54 / 44 with 6 (registers spill), 39 / 32 with twice as
+// many blocks as are resident; 10 and more us longer with units of 2 or 8, or a queue of three units (fewer warps fit).  Backward:
+// 50 with units of 2 and 3 or 4 blocks, 67 with 5, 56 with units of 1, 67 with units of 4.
+constexpr int kForwardUnit = 4, kForwardBlocksPerSm = 5, kBackwardUnit = 2, kBackwardBlocks = 3;
 
 // The units of a warp: the `stride`-th next one each time, without a division.
 struct Walk {
@@ -384,32 +367,38 @@ __global__ void __launch_bounds__(kThreadsN, kForwardBlocksPerSm) norm_rope_kern
         const int kind = kind_of(now.group), base = group_in(now.group, kind) * (U * kSide), first = base + sub;
         const int heads = kind == 0 ? p.q_heads : p.k_heads;
         const int64_t token = now.token;
-        // rows of heads that this warp writes: q_out or k_out, and the token's slot of the cache
-        T* out = kind == 0 ? static_cast<T*>(p.q_out) + (token * p.q_heads + first) * p.dim + run.a
-                 : kind == 1 && p.k_out ? static_cast<T*>(p.k_out) + (token * p.k_heads + first) * p.dim + run.a : nullptr;
-        T* cached = nullptr;
-        int64_t cached_step = 0;
-        if (kind != 0 && p.slots) {
-            const int64_t slot = st.slot[0];
+        // where the unit's heads go, `step` values apart: to q_out or k_out, or to the token's slot of the cache; keys may go to both
+        T* to = kind == 0 ? static_cast<T*>(p.q_out) + (token * p.q_heads + first) * p.dim + run.a : nullptr;
+        T* also = nullptr;
+        int64_t step = kSide * p.dim;
+        if (kind != 0) {
+            if (kind == 1 && p.k_out) also = static_cast<T*>(p.k_out) + (token * p.k_heads + first) * p.dim + run.a;
+            const int64_t slot = p.slots ? st.slot[0] : -1;
             if (slot >= 0 && slot < p.n_slots) {             // (a row without a place in the cache otherwise)
                 const int64_t page = slot >> p.page_shift, at = slot & ((1 << p.page_shift) - 1);
-                cached = (kind == 1 ? static_cast<T*>(p.k_cache) + page * p.k_page + at * p.k_slot + first * p.k_head
-                                    : static_cast<T*>(p.v_cache) + page * p.v_page + at * p.v_slot + first * p.v_head) + run.a;
-                cached_step = kSide * (kind == 1 ? p.k_head : p.v_head);
+                to = (kind == 1 ? static_cast<T*>(p.k_cache) + page * p.k_page + at * p.k_slot + first * p.k_head
+                                : static_cast<T*>(p.v_cache) + page * p.v_page + at * p.v_slot + first * p.v_head) + run.a;
+                step = kSide * (kind == 1 ? p.k_head : p.v_head);
+            } else {
+                to = also;
+                also = nullptr;
             }
+            if (!to) continue;
         }
         // (of the u-th heads side by side, in turn)
         auto store = [&](bool real, const R& a, const R& b) {
-            if (real && out) {
-                *reinterpret_cast<R*>(out) = a;
-                *reinterpret_cast<R*>(out + gap) = b;
+            if (real) {
+                *reinterpret_cast<R*>(to) = a;
+                *reinterpret_cast<R*>(to + gap) = b;
             }
-            if (real && cached) {
-                *reinterpret_cast<R*>(cached) = a;
-                *reinterpret_cast<R*>(cached + gap) = b;
+            to += step;
+            if (also) {
+                if (real) {
+                    *reinterpret_cast<R*>(also) = a;
+                    *reinterpret_cast<R*>(also + gap) = b;
+                }
+                also += kSide * p.dim;
             }
-            if (out) out += kSide * p.dim;
-            cached += cached_step;
         };
         if (kind == 2) {
 #pragma unroll
@@ -433,9 +422,9 @@ __global__ void __launch_bounds__(kThreadsN, kForwardBlocksPerSm) norm_rope_kern
                 const bool real = lane_on && first + u * kSide < heads;
                 Pair v[RUN], y[RUN];
                 unpack_both<T, RUN>(st.runs[2 * u][lane], st.runs[2 * u + 1][lane], real, v);
-                Pair scale = 0;
+                Pair scale{};
                 if (weight) {
-                    Pair ss = 0;
+                    Pair ss{};
 #pragma unroll
                     for (int j = 0; j < RUN; ++j) ss = fma(v[j], v[j], ss);
                     const float rstd = rsqrtf(head_sum<LPH>(sum_of(ss)) * inv + p.eps);
@@ -460,7 +449,7 @@ __global__ void __launch_bounds__(kThreadsN, kForwardBlocksPerSm) norm_rope_kern
 // registers.  Shares are added up in a fixed order: shuffles, the block's warps, and (weight_gradient_kernel) the blocks, so
 // that results repeat bit for bit.
 template <typename T, int RUN, int LPH, int U, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreadsN) norm_rope_backward_kernel(const __grid_constant__ NormRopeBackward p, int q_blocks) {
+__global__ void __launch_bounds__(kThreadsN, kBackwardBlocks) norm_rope_backward_kernel(const __grid_constant__ NormRopeBackward p, int q_blocks) {
     constexpr int kSide = 32 / LPH;
     extern __shared__ __align__(16) uint8_t memory[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l = lane % LPH, sub = lane / LPH;
@@ -538,7 +527,7 @@ __global__ void __launch_bounds__(kThreadsN) norm_rope_backward_kernel(const __g
                 if (turned) y[j] = fma(other[j], partner<RUN, INTERLEAVED>(g, j), y[j]);
             }
             if (weight) {
-                Pair x[RUN], ss = 0, dot = 0;
+                Pair x[RUN], ss{}, dot{};
                 unpack_both<T, RUN>(st.runs[4 * u + 2][lane], st.runs[4 * u + 3][lane], real, x);
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
@@ -619,7 +608,7 @@ constexpr int blocks_per_sm(int most) {
     const int fit = 227 * 1024 / (kWarpsN * kStagesN * int(sizeof(Stage<RUN, LPH, V>)) + 1024);
     return fit < most ? fit : most;
 }
-constexpr int kBackwardBlocksPerSm = blocks_per_sm<8, 16, 4 * kBackwardUnit>(3);
+constexpr int kBackwardBlocksPerSm = blocks_per_sm<8, 16, 4 * kBackwardUnit>(kBackwardBlocks);
 
 template <int RUN, int LPH, int V>
 constexpr int queue_bytes() { return kWarpsN * kStagesN * int(sizeof(Stage<RUN, LPH, V>)); }
@@ -634,7 +623,7 @@ cudaError_t forward(const NormRope& a, int num_sms, cudaStream_t stream) {
     constexpr int U = kForwardUnit, bytes = queue_bytes<RUN, LPH, 2 * U>(), per = U * (32 / LPH);
     const int q_groups = (a.q_heads + per - 1) / per, k_groups = (a.k_heads + per - 1) / per;
     const int groups = q_groups + k_groups + (a.v.data ? k_groups : 0);
-    // (all that are resident, even where fewer would take as many rounds: 41 us against 44)
+    // (all that are resident, even where fewer would take as many rounds: 3 us less)
     const int64_t blocks = (a.tokens * groups + kWarpsN - 1) / kWarpsN, resident = blocks_per_sm<RUN, LPH, 2 * U>(kForwardBlocksPerSm) * num_sms;
     const unsigned grid = unsigned(blocks < resident ? blocks : resident);
     auto kern = a.interleaved ? norm_rope_kernel<T, RUN, LPH, U, true> : norm_rope_kernel<T, RUN, LPH, U, false>;
