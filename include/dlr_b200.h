@@ -216,12 +216,12 @@ DLRB200_API int dlrb200_forward_static(const void* x, void* y, const void* Vp, c
 /* One step's bookkeeping.  For request r, with len = 0 where finished[r] (its
  * pages go back first): the tokens len .. len + new_tokens[r] - 1 get slots, the
  * pages that are missing are taken from the top of the stack free_pages[0 ..
- * n_free), in the order of the requests.  A request is refused, and keeps its
- * length and pages, when it would pass columns pages, when its tokens do not fit
- * its rows, or when it needs pages and those asked for up to and including it
- * are more than there are.  Rows of the batch: `width` per request, or, with
- * width 0, one request behind the other; at most 2^30.  Rows without a token get slot -1 and
- * position 0.  lengths_out and n_free_out may be lengths and n_free. */
+ * n_free), in the order of the requests.  A request is refused, and keeps what
+ * it holds, when it would pass columns pages, when its tokens do not fit its
+ * rows, or when it needs pages and those asked for up to and including it are
+ * more than there are.  Rows of the batch: `width` per request, or, with width
+ * 0, one request behind the other; at most 2^30.  Rows without a token get slot
+ * -1 and position 0.  lengths_out and n_free_out may be lengths and n_free. */
 typedef struct dlrb200_plan_step {
     const int* lengths;             /* (requests) tokens held */
     const int* new_tokens;          /* (requests) */

@@ -115,6 +115,9 @@ bool real(PyObject* o, double* v) {
     return true;
 }
 
+// (a dimension of one has any stride)
+int64_t step_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+
 // ---- plan ------------------------------------------------------------------------------------------------------------------
 // (lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
 PyObject* paged_plan(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
@@ -186,7 +189,7 @@ bool rows_of(const at::Tensor& t, Rows* r) {
         else if (t.stride(i) != r->token * r->tokens) return false;
         r->tokens *= t.size(i);
     }
-    r->head = t.stride(n - 2);
+    r->head = step_of(t, n - 2);
     r->data = t.data_ptr();
     return r->token % 4 == 0 && r->head % 4 == 0 && aligned(t, 8);
 }
@@ -391,7 +394,7 @@ bool cache_of(const at::Tensor& t, int device, at::ScalarType type, int64_t head
     if (!plain(t, device) || t.scalar_type() != type || t.dim() != 4 || t.size(1) != heads || t.size(3) != dim) return false;
     const int64_t page = t.size(2);
     if (page < 16 || page > kMostInt || (page & (page - 1)) || t.size(0) > kMostInt / page) return false;
-    *c = {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+    *c = {t.data_ptr(), step_of(t, 0), step_of(t, 1), t.stride(2)};
     return t.numel() == 0 || (t.stride(3) == 1 && c->page % multiple == 0 && c->head % multiple == 0 && c->slot % multiple == 0 &&
                               aligned(t, uintptr_t(2 * multiple)));
 }
@@ -445,7 +448,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     if ((type != at::kBFloat16 && type != at::kHalf) || (dim != 64 && dim != 96 && dim != 128 && dim != 256) || kv_heads < 1 || heads < 1 ||
         heads % kv_heads || n > kMostInt / heads)
         Py_RETURN_NONE;
-    if (q->numel() > 0 && (q->stride(2) != 1 || q->stride(0) % 2 || q->stride(1) % 2 || !aligned(*q, 4))) Py_RETURN_NONE;
+    if (q->numel() > 0 && (q->stride(2) != 1 || step_of(*q, 0) % 2 || step_of(*q, 1) % 2 || !aligned(*q, 4))) Py_RETURN_NONE;
     Cache kc, vc;
     if (!cache_of(*k_cache, device, type, kv_heads, dim, 8, &kc) || !cache_of(*v_cache, device, type, kv_heads, dim, 8, &vc) ||
         k_cache->sizes() != v_cache->sizes())
@@ -464,7 +467,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
         workspace = at::empty({int64_t(bytes)}, lengths->options().dtype(at::kByte));
     }
     dlrb200_paged_attention_args a{};
-    a.q = q->data_ptr(), a.q_request = q->stride(0), a.q_head = q->stride(1);
+    a.q = q->data_ptr(), a.q_request = step_of(*q, 0), a.q_head = step_of(*q, 1);
     a.k_cache = kc.data, a.kc_page = kc.page, a.kc_head = kc.head, a.kc_slot = kc.slot;
     a.v_cache = vc.data, a.vc_page = vc.page, a.vc_head = vc.head, a.vc_slot = vc.slot;
     a.block_table = as_ints(*table), a.table_stride = table->stride(0), a.lengths = as_ints(*lengths);

@@ -107,7 +107,8 @@ def _check_cache(what, k_cache, v_cache, dtype, kv_heads, dim, multiple):
     if k_cache.shape[0] * k_cache.shape[2] > 0x7fffffff:
         raise ValueError(f"{what}: the caches have more than 2^31 - 1 slots")
     for c in (k_cache, v_cache):
-        if c.numel() and (c.stride(3) != 1 or any(s % multiple for s in c.stride()[:3]) or c.data_ptr() % (2 * multiple)):
+        strides = [s for s, n in zip(c.stride()[:3], c.shape) if n > 1]
+        if c.numel() and (c.stride(3) != 1 or any(s % multiple for s in strides) or c.data_ptr() % (2 * multiple)):
             raise ValueError(f"{what}: the caches need a contiguous last dimension and strides of a multiple of {multiple} elements")
 
 
@@ -131,15 +132,15 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
     request (1: a decode step), or, with ``width=None``, one request behind the other in ``rows`` rows.
 
     ``block_table`` and ``free_pages`` are written in place; lengths and the count of free pages come back as new tensors,
-    or, with ``in_place``, in those given.  A request is refused (its length comes back as it was, its rows have slot -1)
-    when the table has no columns for its tokens, when they do not fit its rows, or when it needs pages and those asked for
+    or, with ``in_place``, in those given.  A request is refused (it keeps its tokens, none if it is finished, and its rows have
+    slot -1) when the table has no columns for its tokens, when they do not fit its rows, or when it needs pages and those asked for
     up to and including it are more than there are free.
     """
     out = _native().paged_plan(lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
     if type(out) is tuple:
         return PagedPlan(*out)
     what = "paged_plan"
-    _all_tensors(what, lengths, new_tokens, block_table, free_pages, n_free)
+    _all_tensors(what, lengths, new_tokens, block_table, free_pages, n_free, *(() if finished is None else (finished,)))
     if lengths.dim() != 1 or block_table.dim() != 2 or free_pages.dim() != 1:
         raise ValueError(f"{what}: expected lengths (requests), block_table (requests, columns), free_pages (pages)")
     n = lengths.shape[0]
@@ -208,6 +209,7 @@ def _check_norm_rope(what, q, k, q_weight, k_weight, cos, sin, positions):
     if positions.shape != q.shape[:-2]:
         raise ValueError(f"{what}: positions have shape {tuple(positions.shape)}, expected {tuple(q.shape[:-2])}")
     given = [w for w in (q_weight, k_weight) if w is not None]
+    _all_tensors(what, *given)
     for w in given:
         if w.dtype not in (q.dtype, torch.float32) or w.dtype != given[0].dtype:
             raise TypeError(f"{what}: the weights have type {w.dtype}, expected {q.dtype} or float32 for both")

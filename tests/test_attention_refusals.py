@@ -44,6 +44,9 @@ def _plan_args(**changed):
     (dict(width=2, rows=5), ValueError),
     (dict(finished=torch.zeros(2, dtype=torch.bool)), ValueError),
     (dict(finished=torch.zeros(3)), ValueError),
+    (dict(finished=[True, False, True]), TypeError),
+    (dict(page_size=2 ** 21), ValueError),
+    (dict(width=None, rows=2 ** 30 + 1), ValueError),
     (dict(lengths=_i32(8193), new_tokens=_i32(8193), block_table=_i32(8193, 1)), ValueError),
 ])
 def test_plan_refuses(changed, error):
@@ -68,6 +71,7 @@ HEADS = [
     (dict(q=torch.zeros(5, 4, 68, dtype=torch.bfloat16), k=torch.zeros(5, 2, 68, dtype=torch.bfloat16)), ValueError),
     (dict(q=torch.zeros(5, 4, 264, dtype=torch.bfloat16), k=torch.zeros(5, 2, 264, dtype=torch.bfloat16)), ValueError),
     (dict(q_weight=torch.ones(32, dtype=torch.bfloat16)), ValueError),
+    (dict(k_weight=1.0), TypeError),
     (dict(q_weight=torch.ones(64, dtype=torch.float16)), TypeError),
     (dict(q_weight=torch.ones(64)), TypeError),                             # one in bf16, one in fp32
     (dict(cos=torch.zeros(9, 40), sin=torch.zeros(9, 40)), ValueError),

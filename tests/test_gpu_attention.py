@@ -477,6 +477,19 @@ def test_attention_orders_and_strides():
     _close(got, *_attend64(q, kc, vc, table, lengths, 0.125))
 
 
+def test_dimensions_of_one_have_any_stride():
+    import dlr_lock_b200 as D
+    kc, vc, table, n = _cache_case([30], 1, 64, 32, torch.bfloat16)
+    odd = [c[:1].as_strided((1, 1, 32, 64), (7, 3, 64, 1)) for c in (kc, vc)]
+    q = _normal(_gen(1), 1, 1, 64, dtype=torch.bfloat16)
+    zero = torch.zeros_like(table)
+    assert torch.equal(D.paged_attention(q.as_strided((1, 1, 64), (5, 9, 1)), *odd, zero, n), D.paged_attention(q, kc[:1], vc[:1], zero, n))
+    cos, sin = D.rope_tables(torch.ones(32, device=DEV), 4)
+    at = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = D.qk_norm_rope_append(q.as_strided((1, 1, 64), (5, 9, 1)), q, q, None, None, cos, sin, at, at + 31, *odd)
+    assert torch.equal(got, q) and torch.equal(kc[0, 0, 31], q[0, 0]) and torch.equal(vc[0, 0, 31], q[0, 0])
+
+
 def test_attention_of_no_requests_no_columns_no_pages():
     import dlr_lock_b200 as D
     kc, vc, table, n = _cache_case([70, 5], 2, 64, 32, torch.bfloat16)
