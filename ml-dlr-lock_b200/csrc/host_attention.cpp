@@ -152,12 +152,19 @@ PyObject* paged_plan(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const at::Tensor all = at::empty({2 * rows + 2 * n + 2}, lengths->options());
-        slots = all.narrow(0, 0, rows);
-        positions = all.narrow(0, rows, rows);
-        starts = all.narrow(0, 2 * rows, n + 1);
+        // vectors over parts of it, made directly (a narrow() costs 0.4 us, five of them a quarter of the call)
+        auto part = [&](int64_t first, int64_t size) {
+            at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+            t.unsafeGetTensorImpl()->set_storage_offset(first);
+            t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+            return t;
+        };
+        slots = part(0, rows);
+        positions = part(rows, rows);
+        starts = part(2 * rows, n + 1);
         const bool in_place = PyObject_IsTrue(o[9]) == 1;
-        lengths_out = in_place ? *lengths : all.narrow(0, 2 * rows + n + 1, n);
-        count_out = in_place ? *count : all.narrow(0, 2 * rows + 2 * n + 1, 1);
+        lengths_out = in_place ? *lengths : part(2 * rows + n + 1, n);
+        count_out = in_place ? *count : part(2 * rows + 2 * n + 1, 1);
     }
     dlrb200_plan_step s{};
     s.lengths = as_ints(*lengths), s.new_tokens = as_ints(*fresh);
