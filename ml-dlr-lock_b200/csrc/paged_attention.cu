@@ -33,6 +33,7 @@ constexpr int kWarpsA = 4;
 constexpr int kThreadsA = 32 * kWarpsA;
 constexpr int kWarpsJ = 8;                       // of the joining kernel
 constexpr int kThreadsJ = 32 * kWarpsJ;
+constexpr int kMostHeads = 64;                   // of a CTA of it
 constexpr int kUnit = 16;                        // tokens of a warp's step
 constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
 // CTAs of an SM for heads of `dim`, nt groups of eight sharing keys: as many as registers and shared memory allow.  More warps
@@ -581,23 +582,25 @@ struct Pieces {
     int parts, run, first_slot, request, head, row;
 };
 
-// Joins the runs over which segments were cut: `per_cta` (1 or 8) query heads to a CTA.  It is launched while the first kernel
-// still runs and finds its place in the work meanwhile.  A warp joins a head of few parts by itself, all warps of the CTA one of
-// many; maxima come first, so that the loads of the parts do not wait for one another.  Sums run in the order of the tokens.
-// (Behind the first kernel it takes 3 us.)
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut, int per_cta) {
+// Joins the runs over which segments were cut: `per_cta` (1, or a multiple of 8 up to 64) query heads to a CTA.  It is launched while
+// the first kernel still runs and finds its place in the work meanwhile.  A warp joins a head of few parts by itself, all warps of the
+// CTA one of many; maxima come first, so that the loads of the parts do not wait for one another.  Sums run in the order of the
+// tokens.  (Behind the first kernel it takes 3 us, 12 for 19200 heads; with eight heads to a CTA those take 24.  A CTA to each run, for
+// the segment that is cut at its end: 7 us more for 2400 heads.)
+template <typename T, int D, int NT, bool MANY>
+__global__ void __launch_bounds__(kThreadsJ, MANY ? 4 : 1) join_kernel(const __grid_constant__ PagedAttention p, int groups, const Cut cut, int per_cta) {
     using S = Shape<D, NT>;
     constexpr int kColumns = (D / 4 + 31) / 32;          // of four values, per lane
-    constexpr int kBatch = 16 / kColumns;                // loads in flight
+    constexpr int kBatch = (MANY ? 8 : 16) / kColumns;   // loads in flight
     constexpr int kFew = 16;
-    __shared__ long long scratch[kWarpsJ], before[kWarpsJ];
+    __shared__ long long scratch[kWarpsJ], before[kMostHeads];
     __shared__ Pieces found[kWarpsJ];
     __shared__ float2 ml[kMostParts];
     __shared__ float highest[kWarpsJ], sums[kWarpsJ];
     __shared__ float4 share[kWarpsJ][D / 4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int group_size = p.heads / p.kv_heads, first_head = int(blockIdx.x) * per_cta, all_heads = p.requests * p.heads;
+    const int group_size = p.heads / p.kv_heads, first_head = int(blockIdx.x) * per_cta;
+    const int last_head = min(p.requests * p.heads - first_head, per_cta) + first_head;
     const Geometry geo{p.lengths, p.requests, p.kv_heads * groups, (long long)p.columns << p.page_shift};
     const int first_request = first_head / p.heads;
     long long total = 0;
@@ -613,25 +616,23 @@ __global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__
         total += here;
     }
     __syncthreads();
-    Pieces mine{};
-    if (warp < per_cta && first_head + warp < all_heads) {
-        const int request = (first_head + warp) / p.heads, head = first_head + warp - request * p.heads;
+    const long long run = cut.run(total);
+    auto pieces_of = [&](int h) {
+        Pieces a{};
+        const int request = h / p.heads, head = h - request * p.heads;
         const int kv_head = head / group_size, in_group = head - kv_head * group_size;
         const int segment = kv_head * groups + in_group / S::kRows;
         const int seg_tiles = (geo.tokens(request) + kTile - 1) / kTile;
         if (seg_tiles) {
-            const long long run = cut.run(total), begin = before[request - first_request] + (long long)segment * seg_tiles;
+            const long long begin = before[request - first_request] + (long long)segment * seg_tiles;
             const int first = int(begin / run), last = int((begin + seg_tiles - 1) / run);
             // the segment opens its first run unless it begins inside it
-            mine = {last - first + 1, first, begin <= run * first ? 0 : 1, request, head, in_group % S::kRows};
+            a = {last - first + 1, first, begin <= run * first ? 0 : 1, request, head, in_group % S::kRows};
         }
-    }
-    if (lane == 0) found[warp] = mine;
-    // The first CTA stays until the first kernel is done, whatever it has to do itself: this kernel then ends after that one,
-    // and what follows on the stream after both.
-    const bool any = __syncthreads_or(mine.parts > 1);
-    if (blockIdx.x == 0 || any) asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!any) return;                                    // nothing was cut
+        return a;
+    };
+    // (every CTA waits for the first kernel, so that this one ends after it, and what follows on the stream after both)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const float* const workspace = static_cast<const float*>(p.workspace);
     auto part_of = [&](const Pieces& a, int i) { return workspace + (int64_t(a.run + i) * 2 + (i == 0 ? a.first_slot : 0)) * S::kPart; };
@@ -669,72 +670,79 @@ __global__ void __launch_bounds__(kThreadsJ) join_kernel(const __grid_constant__
         return x;
     };
 
-    if (mine.parts > 1 && mine.parts <= kFew) {
-        const float2 m = lane < mine.parts ? ml_of(mine, lane) : make_float2(-INFINITY, 0.f);
-        const float top = warp_max(m.x), f = exp2f(m.x - (top == -INFINITY ? 0.f : top)), sum = warp_sum(f * m.y);
-        float4 v[kColumns] = {};
-        for (int i0 = 0; i0 < mine.parts; i0 += kBatch) {
-            float4 x[kBatch][kColumns];
+    for (int h0 = first_head; h0 < last_head; h0 += kWarpsJ) {
+        Pieces mine{};
+        if (h0 + warp < last_head) mine = pieces_of(h0 + warp);
+        if (lane == 0) found[warp] = mine;
+        if (mine.parts > 1 && mine.parts <= kFew) {
+            const float2 m = lane < mine.parts ? ml_of(mine, lane) : make_float2(-INFINITY, 0.f);
+            const float top = warp_max(m.x), f = exp2f(m.x - (top == -INFINITY ? 0.f : top)), sum = warp_sum(f * m.y);
+            float4 v[kColumns] = {};
+            for (int i0 = 0; i0 < mine.parts; i0 += kBatch) {
+                float4 x[kBatch][kColumns];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) load(mine, i0 + i, i0 + i < mine.parts, x[i]);
+                for (int i = 0; i < kBatch; ++i) load(mine, i0 + i, i0 + i < mine.parts, x[i]);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) add(v, __shfl_sync(~0u, f, (i0 + i) & 31), x[i]);      // (0 behind the last part)
-        }
-#pragma unroll
-        for (int k = 0; k < kColumns; ++k)
-            if (k * 32 + lane < D / 4) write(mine, k * 32 + lane, v[k], 1.f / sum);
-    }
-    for (int w = 0; w < per_cta; ++w) {
-        const Pieces a = found[w];
-        if (a.parts <= kFew) continue;
-        float top = -INFINITY;
-        for (int i = threadIdx.x; i < a.parts; i += kThreadsJ) {
-            ml[i] = ml_of(a, i);
-            top = fmaxf(top, ml[i].x);
-        }
-        top = warp_max(top);
-        if (lane == 0) highest[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kWarpsJ; ++k) top = fmaxf(top, highest[k]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const int per = (a.parts + kWarpsJ - 1) / kWarpsJ, lo = warp * per, hi = min(a.parts, lo + per);
-        float4 v[kColumns] = {};
-        float sum = 0.f;
-        for (int i0 = lo; i0 < hi; i0 += kBatch) {
-            float4 x[kBatch][kColumns];
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) load(a, i0 + i, i0 + i < hi, x[i]);
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const float2 m = i0 + i < hi ? ml[i0 + i] : make_float2(-INFINITY, 0.f);
-                const float f = exp2f(m.x - ref);
-                sum += f * m.y;
-                add(v, f, x[i]);
+                for (int i = 0; i < kBatch; ++i) add(v, __shfl_sync(~0u, f, (i0 + i) & 31), x[i]);      // (0 behind the last part)
             }
+#pragma unroll
+            for (int k = 0; k < kColumns; ++k)
+                if (k * 32 + lane < D / 4) write(mine, k * 32 + lane, v[k], 1.f / sum);
         }
-#pragma unroll
-        for (int k = 0; k < kColumns; ++k)
-            if (k * 32 + lane < D / 4) share[warp][k * 32 + lane] = v[k];
-        if (lane == 0) sums[warp] = sum;
-        __syncthreads();
-        sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < kWarpsJ; ++k) sum += sums[k];
-        const float inv = 1.f / sum;
-        for (int c = threadIdx.x; c < D / 4; c += kThreadsJ) {
-            float4 x = share[0][c];
-#pragma unroll
-            for (int k = 1; k < kWarpsJ; ++k) {
-                const float4 y = share[k][c];
-                x.x += y.x;
-                x.y += y.y;
-                x.z += y.z;
-                x.w += y.w;
+        if (!__syncthreads_or(mine.parts > kFew)) continue;
+        for (int w = 0; w < kWarpsJ; ++w) {
+            const Pieces a = found[w];
+            if (a.parts <= kFew) continue;
+            float top = -INFINITY;
+            for (int i = threadIdx.x; i < a.parts; i += kThreadsJ) {
+                ml[i] = ml_of(a, i);
+                top = fmaxf(top, ml[i].x);
             }
-            write(a, c, x, inv);
+            top = warp_max(top);
+            if (lane == 0) highest[warp] = top;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < kWarpsJ; ++k) top = fmaxf(top, highest[k]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            const int per = (a.parts + kWarpsJ - 1) / kWarpsJ, lo = warp * per, hi = min(a.parts, lo + per);
+            float4 v[kColumns] = {};
+            float sum = 0.f;
+            for (int i0 = lo; i0 < hi; i0 += kBatch) {
+                float4 x[kBatch][kColumns];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) load(a, i0 + i, i0 + i < hi, x[i]);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const float2 m = i0 + i < hi ? ml[i0 + i] : make_float2(-INFINITY, 0.f);
+                    const float f = exp2f(m.x - ref);
+                    sum += f * m.y;
+                    add(v, f, x[i]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kColumns; ++k)
+                if (k * 32 + lane < D / 4) share[warp][k * 32 + lane] = v[k];
+            if (lane == 0) sums[warp] = sum;
+            __syncthreads();
+            sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarpsJ; ++k) sum += sums[k];
+            const float inv = 1.f / sum;
+            for (int c = threadIdx.x; c < D / 4; c += kThreadsJ) {
+                float4 x = share[0][c];
+#pragma unroll
+                for (int k = 1; k < kWarpsJ; ++k) {
+                    const float4 y = share[k][c];
+                    x.x += y.x;
+                    x.y += y.y;
+                    x.z += y.z;
+                    x.w += y.w;
+                }
+                write(a, c, x, inv);
+            }
+            __syncthreads();                                 // the next head's turn
         }
-        __syncthreads();                                 // the next head's turn
+        __syncthreads();                                     // everyone has read what was found
     }
 }
 
@@ -776,13 +784,17 @@ cudaError_t launch(const PagedAttention& a, int num_sms, cudaStream_t stream) {
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     // a head to a CTA while that is a few CTAs for each SM at most
-    const int per_cta = int64_t(a.requests) * a.heads <= 4 * num_sms ? 1 : kWarpsJ;
-    cfg.gridDim = dim3((unsigned(a.requests) * unsigned(a.heads) + per_cta - 1) / per_cta);
+    // (and as many as keep it so, beyond)
+    const long long heads = (long long)a.requests * a.heads, most_ctas = 4 * num_sms;
+    long long per = heads <= most_ctas ? 1 : (heads + most_ctas - 1) / most_ctas;
+    if (per > 1) per = (per + kWarpsJ - 1) / kWarpsJ * kWarpsJ;
+    const int per_cta = int(per < kMostHeads ? per : kMostHeads);
+    cfg.gridDim = dim3(unsigned((heads + per_cta - 1) / per_cta));
     cfg.blockDim = dim3(kThreadsJ);
     cfg.stream = stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, groups, cut, per_cta);
+    return cudaLaunchKernelEx(&cfg, per_cta > 1 ? join_kernel<T, D, NT, true> : join_kernel<T, D, NT, false>, a, groups, cut, per_cta);
 }
 
 template <typename T, int D>

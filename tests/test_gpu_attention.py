@@ -445,6 +445,13 @@ def test_attention_many_requests(requests, columns):
     _check_attention([rng.choice([0, 1, rng.randint(0, 700)]) for _ in range(requests)], 6, 2, 64, 16, "fp16", columns=columns)
 
 
+def test_attention_long_and_short_requests_of_many_heads():
+    # heads of hundreds of parts beside heads of few and of one, several rounds of heads to a CTA of the join
+    lengths = [30000, 3, 0, 700, 9000, 1] * 3 + [50] * 30
+    _check_attention(lengths, 64, 2, 64, 64, "bf16")
+    _check_attention([20000, 0, 40], 32, 1, 128, 16, "fp16")
+
+
 @pytest.mark.parametrize("columns", [9, 900])
 @pytest.mark.parametrize("fill", [float("nan"), float("inf"), -65504.0])
 def test_attention_never_reads_what_no_request_holds(fill, columns):
