@@ -1,6 +1,6 @@
 // Host side of the attention operators, native because a decode step calls them for every layer and the kernels of a small
 // batch take 3 us: checks, outputs and argument structs cost 20 to 40 us per call in Python (197 us for a training step with
-// its Python autograd function), about 4 here.
+// its Python autograd function), about 6 here with the launch.
 //
 //   bind(addresses)          the C-ABI functions to call, in the order of Library
 //   paged_plan(...), qk_norm_rope(...), qk_norm_rope_append(...), paged_attention(...)
