@@ -67,7 +67,8 @@ class PagedDecoder:
 
     ``admit`` takes prompts, ``step`` one token per request; both return the logits of the last token of every request
     that has one.  A request that could not be given its tokens (no free pages, or ``max_tokens`` reached) keeps its length
-    (``cache.lengths``), and its row of logits is NaN, as is that of a request without a token.
+    (``cache.lengths``; none, where a new prompt was to replace it), and its row of logits is NaN, as is that of a request
+    without a token.
     """
 
     def __init__(self, model, requests: int, max_tokens: int, *, pages: Optional[int] = None, page_size: int = 64):
@@ -102,15 +103,19 @@ class PagedDecoder:
             h = layer.mlp.dlrnet(h + attn.o_proj(out.flatten(1)))
         return h
 
+    def _embed(self, ids, plan):
+        """Embeddings of the rows that have a token; what stands in the others' ids is not looked up."""
+        return self.model.model.embed_tokens(ids.flatten().masked_fill(plan.slots < 0, 0))
+
     def _logits(self, h, has_token):
         logits = self.model.lm_head(self.model.model.norm(h))
         return logits.masked_fill(~has_token[:, None], float("nan"))
 
     @torch.no_grad()
     def admit(self, ids: torch.Tensor, counts: torch.Tensor, finished: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """New prompts: ``ids`` (requests, width), of which the first ``counts`` (requests, int32) of each row count.  A
-        request with a prompt loses what it held; one with a count of 0 keeps it, unless ``finished`` (requests, bool) gives
-        its pages back.  Returns logits (requests, vocabulary)."""
+        """New prompts: ``ids`` (requests, width), of which the first ``counts`` (requests, int32) of each row count; the
+        others may be anything.  A request with a prompt loses what it held; one with a count of 0 keeps it, unless
+        ``finished`` (requests, bool) gives its pages back.  Returns logits (requests, vocabulary)."""
         cache = self.cache
         if ids.dim() != 2 or ids.shape[0] != cache.requests or ids.shape[1] < 1:
             raise ValueError(f"admit: expected ids ({cache.requests}, width), got {tuple(ids.shape)}")
@@ -127,15 +132,15 @@ class PagedDecoder:
             out = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=attn.scaling, enable_gqa=True)
             return out.transpose(1, 2).flatten(0, 1)
 
-        h = self._layers(self.model.model.embed_tokens(ids).flatten(0, 1), plan, attend)
+        h = self._layers(self._embed(ids, plan), plan, attend)
         first = torch.arange(cache.requests, device=ids.device) * width
         last = first + (counts.long().clamp(1, width) - 1)
         return self._logits(h[last], (counts > 0) & (plan.slots[first] >= 0))
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, active: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """One token of every request, ``tokens`` (requests), or of those marked in ``active`` (requests, bool); returns
-        logits (requests, vocabulary)."""
+        """One token of every request, ``tokens`` (requests), or of those marked in ``active`` (requests, bool; the others'
+        may be anything); returns logits (requests, vocabulary)."""
         cache = self.cache
         if tokens.shape != (cache.requests,):
             raise ValueError(f"step: expected tokens ({cache.requests},), got {tuple(tokens.shape)}")
@@ -145,7 +150,7 @@ class PagedDecoder:
             q = attention.qk_norm_rope_append(q, k, v, *where, eps=eps)
             return attention.paged_attention(q, where[-2], where[-1], cache.block_table, cache.lengths, scale=attn.scaling)
 
-        h = self._layers(self.model.model.embed_tokens(tokens), plan, attend)
+        h = self._layers(self._embed(tokens, plan), plan, attend)
         return self._logits(h, plan.slots >= 0)
 
     def capture(self):
@@ -172,4 +177,5 @@ class PagedDecoder:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=side):
                 logits = self.step(tokens)
+        graph.decoder = self                 # (a replay reads its cache and its tables)
         return graph, tokens, logits

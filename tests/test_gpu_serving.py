@@ -105,6 +105,44 @@ def test_pages_run_out_and_come_back():
         decoder.admit(ids[:2], i32([1, 1, 1]))
 
 
+def test_ids_behind_a_prompt_and_of_inactive_requests_may_be_anything():
+    import dlr_lock_b200 as D
+    model = _model(layers=2)
+    ids = torch.randint(0, 1000, (3, 20), device=DEV)
+    counts = torch.tensor([20, 7, 0], dtype=torch.int32, device=DEV)
+    active = torch.tensor([True, False, False], device=DEV)
+    runs = []
+    for fill in (0, -100, 1 << 40):
+        decoder = D.PagedDecoder(model, requests=3, max_tokens=64)
+        padded = ids.masked_fill(torch.arange(20, device=DEV) >= counts[:, None], fill)
+        first = decoder.admit(padded, counts)
+        runs.append((first[:2], decoder.step(ids[:, 0].masked_fill(~active, fill), active)[:1]))
+    assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(runs[0], run))
+    assert all(torch.isfinite(t).all() for t in runs[0])
+
+
+def test_a_captured_step_keeps_its_cache():
+    import dlr_lock_b200 as D
+    model = _model(layers=1)
+    ids = torch.randint(0, 1000, (2, 9), device=DEV)
+
+    def start():
+        decoder = D.PagedDecoder(model, requests=2, max_tokens=64)
+        decoder.admit(ids, torch.tensor([9, 4], dtype=torch.int32, device=DEV))
+        return decoder
+
+    def replayed(graph, tokens, logits):
+        tokens.copy_(ids[:, 0])
+        graph.replay()
+        return logits.clone()
+
+    held = start()
+    want = replayed(*held.capture())
+    captured = start().capture()                             # (nothing else holds this decoder)
+    others = [torch.full((1 << 20,), float("nan"), device=DEV) for _ in range(8)]
+    assert torch.equal(replayed(*captured), want) and all(torch.isnan(t).all() for t in others)
+
+
 def test_what_the_decoder_refuses():
     import dlr_lock_b200 as D
     model = _model(layers=1)
