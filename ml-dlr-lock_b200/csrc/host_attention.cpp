@@ -188,16 +188,20 @@ struct Rows {
 bool rows_of(const at::Tensor& t, Rows* r) {
     const int64_t n = t.dim();
     if (n < 2 || (t.stride(n - 1) != 1 && t.size(n - 1) > 1)) return false;
+    r->data = t.data_ptr();
+    r->head = step_of(t, n - 2);
     r->tokens = 1;
     r->token = 0;
+    if (t.numel() == 0) {                    // (no strides to agree on)
+        r->tokens = r->head = 0;
+        return true;
+    }
     for (int64_t i = n - 3; i >= 0; --i) {
         if (t.size(i) == 1) continue;
         if (r->tokens == 1) r->token = t.stride(i);
         else if (t.stride(i) != r->token * r->tokens) return false;
         r->tokens *= t.size(i);
     }
-    r->head = step_of(t, n - 2);
-    r->data = t.data_ptr();
     return r->token % 4 == 0 && r->head % 4 == 0 && aligned(t, 8);
 }
 

@@ -293,6 +293,21 @@ def test_norm_rope_of_no_tokens_of_layouts_that_are_copied_and_twice():
         torch.autograd.grad(once.float().sum(), leaf)
 
 
+@pytest.mark.parametrize("lead", [(2, 0), (0, 2), (2, 0, 3), (0,)])
+def test_norm_rope_of_empty_batches(lead):
+    import dlr_lock_b200 as D
+    q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(1, 4, 2, 64, 32, torch.bfloat16, False, True)
+    empty = [t.new_empty(*lead, *t.shape[1:]) for t in (q, k, v)]
+    where = torch.empty(lead, dtype=torch.int32, device=DEV)
+    leaves = [t.detach().requires_grad_(True) for t in (empty[0], empty[1], qw, kw)]
+    out = D.qk_norm_rope(*leaves, cos, sin, where)
+    got = torch.autograd.grad(out, leaves, [torch.zeros_like(o) for o in out])
+    assert [g.shape for g in got] == [t.shape for t in leaves] and out[0].shape == empty[0].shape and out[1].shape == empty[1].shape
+    assert not got[2].any() and not got[3].any()
+    cache = torch.zeros(1, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    assert D.qk_norm_rope_append(*empty, qw, kw, cos, sin, where, where, cache, cache.clone()).shape == empty[0].shape
+
+
 def test_norm_rope_gradient_captured():
     import dlr_lock_b200 as D
     q, k, _, qw, kw, cos, sin, positions = _norm_rope_case(200, 8, 2, 128, 64, torch.bfloat16, False, True)
