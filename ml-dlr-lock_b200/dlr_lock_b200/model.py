@@ -326,10 +326,14 @@ class RotaryTables:
 
     def on(self, device):
         device = torch.device(device)
-        if device not in self._made:
-            scale = float(getattr(self._rotary, "attention_scaling", 1.0))
-            self._made[device] = attention.rope_tables(self._rotary.inv_freq.detach().to(device), self._positions, scale)
-        return self._made[device]
+        if device in self._made:
+            return self._made[device]
+        scale = float(getattr(self._rotary, "attention_scaling", 1.0))
+        with torch.inference_mode(False):        # (a later training step saves them for its gradient)
+            made = attention.rope_tables(self._rotary.inv_freq.detach().to(device), self._positions, scale)
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+            self._made[device] = made            # (a graph's hold nothing before its first replay: they stay its own)
+        return made
 
 
 def head_norms(attn):

@@ -214,3 +214,34 @@ def test_fused_attention_modules_decode_on_the_host_caches():
         D.fuse_decoder_layers(model, True)
         want = D.evaluate_ppl(model, D.synthetic_token_stream(1000, 64, 2, seed=1), n_steps=2, device=DEV)
     assert abs(ppl / want - 1) <= 1e-2
+
+
+def test_fused_attention_modules_first_used_in_inference_mode_or_in_a_capture():
+    import dlr_lock_b200 as D
+    model = _model(layers=2)
+    ids = torch.randint(0, 1000, (2, 24), device=DEV)
+    with torch.no_grad():
+        D.fuse_decoder_layers(model, True, attention=True)
+        want = model(ids).logits                             # (and everything else that a first call makes)
+
+    D.fuse_decoder_layers(model, True, attention=True)       # the tables anew
+    with torch.inference_mode():
+        assert torch.equal(model(ids).logits, want)
+    model.train()
+    out = model(ids).logits
+    out.float().square().mean().backward()
+    grads = [layer.self_attn.q_norm.weight.grad for layer in model.model.layers]
+    assert all(g is not None and torch.isfinite(g).all() for g in grads)
+    model.eval()
+
+    q, k = (torch.randn(2, 24, n, 128, device=DEV).to(torch.bfloat16) for n in (8, 4))
+    positions = torch.arange(24, device=DEV).expand(2, 24)
+    tables = model.model.layers[0].self_attn._rotary_tables
+    truth = D.qk_norm_rope(q, k, None, None, *tables.on(q.device), positions)
+    fresh = type(tables)(model)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = D.qk_norm_rope(q, k, None, None, *fresh.on(q.device), positions)
+    eager = D.qk_norm_rope(q, k, None, None, *fresh.on(q.device), positions)      # before any replay
+    graph.replay()
+    assert all(torch.equal(a, b) and torch.equal(c, b) for a, b, c in zip(eager, truth, captured))
