@@ -21,20 +21,13 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 EPS = 1e-6
 
 
-_attention = None
-
-
 def _api():
-    """The framework's entry points, imported once, as a program imports them."""
-    global _attention
-    if _attention is None:
-        path = os.path.join(os.getcwd(), "ml-dlr-lock_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        from dlr_lock_b200 import attention
+    path = os.path.join(os.getcwd(), "ml-dlr-lock_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from dlr_lock_b200 import attention
 
-        _attention = attention
-    return _attention
+    return attention
 
 
 def _plan(name, requests, longest, page, width, growing):
