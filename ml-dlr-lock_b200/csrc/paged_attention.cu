@@ -17,7 +17,8 @@
 // output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  Scores are (heads x tokens), the
 // output is turned round, (values x heads): the scores' registers then are the second product's operand as they are, and the
 // output of eight heads takes half the registers that 16 rows would.  Softmax weights enter that product as the sum of two 16-bit
-// terms, so that their rounding (2^-16) does not show in the result.
+// terms, so that their rounding (2^-16) does not show in the result.  fp16 ends 2^-24 below 1, which a long tail of tokens beside
+// one large weight would feel: there the terms are those of the weight times 2^15, and the output is brought back at the end.
 #include "paged_attention.h"
 
 #include <cuda_bf16.h>
@@ -55,6 +56,10 @@ constexpr int kShort = 12;
 constexpr int kMostSms = 160;
 constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
+// What the weights (1 at most) are multiplied by before they are split in two 16-bit terms.  bf16 reaches as far down as fp32; in
+// fp16, with 2^15, a weight is right to 2^-16 of itself down to 2^-24 of the largest one, and to 2^-40 of the largest one below.
+template <typename T>
+constexpr float kWeightUp = __is_same(T, __half) ? 32768.f : 1.f;
 
 template <int D, int NT>
 struct Shape {
@@ -449,8 +454,8 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - ref);
                 l[n] = l[n] * alpha[n] + ((x[0] + x[1]) + (x[2] + x[3]));
-                split2<T>(x[0], x[1], hi[n][0], lo[n][0]);
-                split2<T>(x[2], x[3], hi[n][1], lo[n][1]);
+                split2<T>(x[0] * kWeightUp<T>, x[1] * kWeightUp<T>, hi[n][0], lo[n][0]);
+                split2<T>(x[2] * kWeightUp<T>, x[3] * kWeightUp<T>, hi[n][1], lo[n][1]);
             }
             bool same = alpha[0] == 1.f;
             if constexpr (NT == 2) same = same && alpha[1] == 1.f;
@@ -529,7 +534,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 *reinterpret_cast<float2*>(join + row * S::kJoinRow + c) = v;
                 if (c == 0) share_ml[row] = make_float2(top, sum);
             } else if (whole) {
-                const float inv = 1.f / sum;
+                const float inv = 1.f / kWeightUp<T> / sum;
                 *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(piece.request) * p.heads + out_head + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
             } else {
                 *reinterpret_cast<float2*>(part + row * D + c) = v;
@@ -562,7 +567,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                     v.x += f * x[w].x;
                     v.y += f * x[w].y;
                 }
-                const float inv = piece.tokens ? 1.f / sum : 0.f;        // (no tokens: zeros)
+                const float inv = piece.tokens ? 1.f / kWeightUp<T> / sum : 0.f;        // (no tokens: zeros)
                 *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (int64_t(piece.request) * p.heads + out_head + row) * D + c) = pack2<T>(v.x * inv, v.y * inv);
             }
             __syncwarp();
@@ -687,7 +692,7 @@ __global__ void __launch_bounds__(kThreadsJ, MANY ? 4 : 1) join_kernel(const __g
             }
 #pragma unroll
             for (int k = 0; k < kColumns; ++k)
-                if (k * 32 + lane < D / 4) write(mine, k * 32 + lane, v[k], 1.f / sum);
+                if (k * 32 + lane < D / 4) write(mine, k * 32 + lane, v[k], 1.f / kWeightUp<T> / sum);
         }
         if (!__syncthreads_or(mine.parts > kFew)) continue;
         for (int w = 0; w < kWarpsJ; ++w) {
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(kThreadsJ, MANY ? 4 : 1) join_kernel(const __g
             sum = 0.f;
 #pragma unroll
             for (int k = 0; k < kWarpsJ; ++k) sum += sums[k];
-            const float inv = 1.f / sum;
+            const float inv = 1.f / kWeightUp<T> / sum;
             for (int c = threadIdx.x; c < D / 4; c += kThreadsJ) {
                 float4 x = share[0][c];
 #pragma unroll
