@@ -16,9 +16,8 @@
 // (cp.async, rows padded by 16 bytes so that ldmatrix meets no bank twice), multiplies with mma.sync, and keeps maximum, sum and
 // output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  Scores are (heads x tokens), the
 // output is turned round, (values x heads): the scores' registers then are the second product's operand as they are, and the
-// output of eight heads takes half the registers that 16 rows would.  Softmax weights enter that product as the sum of two 16-bit
-// terms, so that their rounding (2^-16) does not show in the result.  fp16 ends 2^-24 below 1, which a long tail of tokens beside
-// one large weight would feel: there the terms are those of the weight times 2^15, and the output is brought back at the end.
+// output of eight heads takes half the registers that 16 rows would.  A softmax weight enters that product as a sum of 16-bit terms,
+// three in bf16 (all 24 bits of it), two in fp16 (22 bits).
 #include "paged_attention.h"
 
 #include <cuda_bf16.h>
@@ -56,10 +55,15 @@ constexpr int kShort = 12;
 constexpr int kMostSms = 160;
 constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
-// What the weights (1 at most) are multiplied by before they are split in two 16-bit terms.  bf16 reaches as far down as fp32; in
-// fp16, with 2^15, a weight is right to 2^-16 of itself down to 2^-24 of the largest one, and to 2^-40 of the largest one below.
+// What the weights (1 at most) are multiplied by before they are split in terms; the output is brought back at the end.  bf16 reaches as
+// far down as fp32.  fp16 ends 2^-24 below 1, which a long tail of tokens beside one large weight would feel: with 2^15 a weight is
+// right to 2^-16 of itself down to 2^-24 of the largest one, to 2^-40 of the largest one down to 2^-39 of it, and to 2^-38 below.
 template <typename T>
 constexpr float kWeightUp = __is_same(T, __half) ? 32768.f : 1.f;
+template <typename T>
+constexpr int kTerms = __is_same(T, __half) ? 2 : 3;
+template <typename T>
+constexpr float kLeastTerm = __is_same(T, __half) ? 0x1p-24f : 0x1p-126f;
 
 template <int D, int NT>
 struct Shape {
@@ -108,19 +112,19 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
     }
 }
 
-// two values rounded to 16 bits, and what that left over, rounded likewise
+// two values in 16 bits, rounded toward zero
 template <typename T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    if constexpr (__is_same(T, __half)) {
-        const __half2 h = __floats2half2_rn(x, y);
-        const float2 f = __half22float2(h);
-        const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-        hi = *reinterpret_cast<const uint32_t*>(&h);
-        lo = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-        hi = pack_bf16x2(x, y);
-        lo = pack_bf16x2(x - bf16lo_to_f(hi), y - bf16hi_to_f(hi));
-    }
+__device__ __forceinline__ uint32_t toward_zero2(float x, float y) {
+    uint32_t v;
+    if constexpr (__is_same(T, __half)) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
+    else v = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 floats2(uint32_t v) {
+    if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return make_float2(bf16lo_to_f(v), bf16hi_to_f(v));
 }
 
 template <typename T>
@@ -130,6 +134,28 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
         return *reinterpret_cast<const uint32_t*>(&h);
     } else {
         return pack_bf16x2(x, y);
+    }
+}
+
+// Two weights as sums of 16-bit terms.  All terms of a weight above 0 are above 0: a term that is zero or negative would turn an
+// infinite value into NaN or the other infinity, by the weight's bits.  Hence the rounding toward zero; the last term takes what is left.
+// (Two terms of bf16 leave outputs 1e-4 away from those of fp32 weights, three 5e-5, which is what sums in another order do.  64
+// ragged requests of up to 8000 tokens: 164.4 us with two terms, 165.1 with three; one of 131072: 91.8 and 93.0; 64 of up to 4000, 16
+// heads of 64 to a key head: 65.8 and 73.1.  Two signed terms, and the tokens once more where an output is not finite: 166.3, 93.0, 69.3.)
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&term)[kTerms<T>]) {
+    const float least_x = x > 0.f ? kLeastTerm<T> : 0.f, least_y = y > 0.f ? kLeastTerm<T> : 0.f;
+    if constexpr (__is_same(T, __half)) {      // (half of the least term less: together the two are off by as much up as down)
+        term[0] = toward_zero2<T>(fmaxf(x - kLeastTerm<T> / 2, least_x), fmaxf(y - kLeastTerm<T> / 2, least_y));
+    } else {
+        term[0] = toward_zero2<T>(x, y);
+    }
+#pragma unroll
+    for (int i = 1; i < kTerms<T>; ++i) {
+        const float2 before = floats2<T>(term[i - 1]);
+        x = fmaxf(x - before.x, least_x);
+        y = fmaxf(y - before.y, least_y);
+        term[i] = i + 1 < kTerms<T> ? toward_zero2<T>(x, y) : pack2<T>(x, y);
     }
 }
 
@@ -434,7 +460,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
             }
             const int valid = tokens - (first + step * kWarpsA) * kUnit;
             float alpha[NT];
-            uint32_t hi[NT][2], lo[NT][2];
+            uint32_t weight[NT][2][kTerms<T>];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float x[4];
@@ -454,8 +480,8 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - ref);
                 l[n] = l[n] * alpha[n] + ((x[0] + x[1]) + (x[2] + x[3]));
-                split2<T>(x[0] * kWeightUp<T>, x[1] * kWeightUp<T>, hi[n][0], lo[n][0]);
-                split2<T>(x[2] * kWeightUp<T>, x[3] * kWeightUp<T>, hi[n][1], lo[n][1]);
+                split2<T>(x[0] * kWeightUp<T>, x[1] * kWeightUp<T>, weight[n][0]);
+                split2<T>(x[2] * kWeightUp<T>, x[3] * kWeightUp<T>, weight[n][1]);
             }
             bool same = alpha[0] == 1.f;
             if constexpr (NT == 2) same = same && alpha[1] == 1.f;
@@ -479,9 +505,9 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 uint32_t a0, a1, a2, a3;
                 ldmatrix_x4_trans(v_at + t * 32, a0, a1, a2, a3);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                for (int i = 0; i < kTerms<T>; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+                    for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, weight[n][0][i], weight[n][1][i]);
             }
         }
         const int out_head = head0, out_rows = rows;
