@@ -76,6 +76,13 @@ void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(c10::Device
 
 int* as_ints(const at::Tensor& t) { return static_cast<int*>(t.data_ptr()); }
 
+// Whether one carries a tangent of forward-mode differentiation, which no_grad leaves on.
+bool has_tangent(std::initializer_list<const at::Tensor*> tensors) {
+    for (const at::Tensor* t : tensors)
+        if (t && t->defined() && t->_fw_grad(0).defined()) return true;
+    return false;
+}
+
 bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
     if (!at::GradMode::is_enabled()) return false;
     for (const at::Tensor* t : tensors)
@@ -253,7 +260,7 @@ struct Heads {
             any = true;
         }
         weights_f32 = any && type_of_weights == at::kFloat;
-        return !wants_grad({&cos, &sin});
+        return !wants_grad({&cos, &sin}) && !has_tangent({&q, &k, &q_weight, &k_weight, &cos, &sin});
     }
 
     dlrb200_norm_rope_args args() const {
@@ -418,7 +425,7 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n_args) 
     const at::Tensor *v = tensor(o[7]), *slots = tensor(o[8]), *k_cache = tensor(o[9]), *v_cache = tensor(o[10]);
     if (!v || !slots || !k_cache || !v_cache) Py_RETURN_NONE;
     h.interleaved = PyObject_IsTrue(o[12]) == 1;
-    if (!h.check() || wants_grad({&h.q, &h.k, v, &h.q_weight, &h.k_weight, k_cache, v_cache})) Py_RETURN_NONE;
+    if (!h.check() || wants_grad({&h.q, &h.k, v, &h.q_weight, &h.k_weight, k_cache, v_cache}) || has_tangent({v, k_cache, v_cache})) Py_RETURN_NONE;
     Rows v_rows;
     Cache kc, vc;
     const int64_t n = h.q.dim(), kv_heads = h.k.size(n - 2);
@@ -453,7 +460,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     const at::Tensor *q = tensor(o[0]), *k_cache = tensor(o[1]), *v_cache = tensor(o[2]), *table = tensor(o[3]), *lengths = tensor(o[4]);
     if (!q || !k_cache || !v_cache || !table || !lengths) Py_RETURN_NONE;
     const int device = device_of(q);
-    if (device < 0 || !plain(*q, device) || q->dim() != 3 || k_cache->dim() != 4 || wants_grad({q, k_cache, v_cache})) Py_RETURN_NONE;
+    if (device < 0 || !plain(*q, device) || q->dim() != 3 || k_cache->dim() != 4 || wants_grad({q, k_cache, v_cache}) ||
+        has_tangent({q, k_cache, v_cache}))
+        Py_RETURN_NONE;
     const auto type = q->scalar_type();
     const int64_t n = q->size(0), heads = q->size(1), dim = q->size(2), kv_heads = k_cache->size(1);
     if ((type != at::kBFloat16 && type != at::kHalf) || (dim != 64 && dim != 96 && dim != 128 && dim != 256) || kv_heads < 1 || heads < 1 ||

@@ -19,6 +19,7 @@ import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import EPS
@@ -78,6 +79,11 @@ def _on_one_device(what, *tensors):
         elif t.device != device:
             raise ValueError(f"{what}: tensors on {device} and {t.device}")
     return device
+
+
+def _no_tangents(what, *tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _int32(what, name, t, shape):
@@ -239,7 +245,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     ``q_weight`` and ``k_weight`` (dim), in the heads' type or fp32; None leaves that norm out.  ``cos`` and ``sin``
     (positions, half) fp32, see ``rope_tables``: the first 2 * half values of a head are turned, in pairs (i, i + half), or
     (2i, 2i + 1) with ``interleaved``; the rest passes through.  ``positions`` (...) int32 or int64; one outside the tables
-    makes its row NaN.  fp32 throughout, rounded once.  Differentiable (once) in q, k and the weights.
+    makes its row NaN.  fp32 throughout, rounded once.  Differentiable (once, in reverse mode) in q, k and
+    the weights.
     """
     out = _native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
     if type(out) is tuple:
@@ -248,6 +255,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     _check_norm_rope(what, q, k, q_weight, k_weight, cos, sin, positions)
     if cos.requires_grad or sin.requires_grad:
         raise ValueError(f"{what}: the tables have no gradient")
+    _no_tangents(what, q, k, q_weight, k_weight, cos, sin)
     device = _on_one_device(what, q, k, q_weight, k_weight, cos, sin, positions)
     with torch.cuda.device(device):
         out = _native().qk_norm_rope(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), float(eps), bool(interleaved))
@@ -277,6 +285,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     _check_cache(what, k_cache, v_cache, q.dtype, k.shape[-2], dim, 4)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight, k_cache, v_cache)):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    _no_tangents(what, q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)
     device = _on_one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache)
     with torch.cuda.device(device):
         out = _native().qk_norm_rope_append(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), _heads(v, 4), slots.contiguous(),
@@ -320,6 +329,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"{what}: a request of more than 2^30 tokens")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    _no_tangents(what, q, k_cache, v_cache)
     device = _on_one_device(what, q, k_cache, v_cache, block_table, lengths)
     with torch.cuda.device(device):
         out = _native().paged_attention(_heads(q, 2), k_cache, v_cache, block_table, lengths, None if scale is None else float(scale))

@@ -1,0 +1,25 @@
+"""Calls of the attention operators that are refused by name rather than answered wrongly, on the CPU."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import dlr_lock_b200 as D
+from test_attention_refusals import _append_args, _attention_args, _heads_args
+
+
+@pytest.mark.parametrize("call,args,names", [
+    (D.qk_norm_rope, _heads_args, ("q", "k", "q_weight", "k_weight", "cos")),
+    (D.qk_norm_rope_append, _append_args, ("q", "k", "v", "q_weight", "sin", "k_cache")),
+    (D.paged_attention, _attention_args, ("q", "k_cache", "v_cache")),
+])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(call, args, names, grad):
+    # a tangent would be dropped without a word (torch.no_grad() does not switch forward mode off)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        for name in names:
+            given = args()
+            given[name] = forward_ad.make_dual(given[name], torch.ones_like(given[name]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(**given)
+        with pytest.raises(ValueError, match="CUDA"):              # (no tangent: the next check)
+            call(**args())

@@ -1,0 +1,31 @@
+"""Calls of the attention operators as programs make them around the edges: forward-mode tensors, odd gradients, other layouts."""
+import pytest
+import torch
+
+from test_gpu_attention import DEV, _cache_case, _gen, _norm_rope_case, _normal
+
+pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_derivatives_are_refused():
+    import dlr_lock_b200 as D
+    import torch.autograd.forward_ad as forward_ad
+    q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(9, 4, 2, 64, 32, torch.bfloat16, False, True)
+    kc, vc, table, n = _cache_case([40], 2, 64, 32, torch.bfloat16)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for args in ((dual(q), k, qw, kw, cos, sin), (q, dual(k), qw, kw, cos, sin), (q, k, qw, dual(kw), cos, sin), (q, k, qw, kw, dual(cos), sin)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                D.qk_norm_rope(*args, positions)
+        slots = torch.arange(9, dtype=torch.int32, device=DEV)
+        for values, cache in ((dual(v), vc), (v, dual(vc))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                D.qk_norm_rope_append(q, k, values, qw, kw, cos, sin, positions, slots, kc, cache)
+        row = _normal(_gen(0), 1, 4, 64, dtype=torch.bfloat16)
+        for args in ((dual(row), kc, vc), (row, dual(kc), vc), (row, kc, dual(vc))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                D.paged_attention(*args, table, n)
+        D.qk_norm_rope(q, k, qw, kw, cos, sin, positions)          # (without a tangent all is as ever)
+        D.paged_attention(row, kc, vc, table, n)
