@@ -311,7 +311,7 @@ def _fused_locked_layer_forward(self, hidden_states, **kwargs):
 
 class RotaryTables:
     """Cosines and sines of a decoder's rotary embedding for every position up to its ``max_position_embeddings`` (or ``positions``),
-    fp32, made on first use on each device."""
+    fp32, made on first use on each device.  Once made they are there for every stream and thread: the first use waits for them."""
 
     def __init__(self, model, positions: Optional[int] = None):
         self._rotary = model.model.rotary_emb
@@ -331,8 +331,11 @@ class RotaryTables:
         scale = float(getattr(self._rotary, "attention_scaling", 1.0))
         with torch.inference_mode(False):        # (a later training step saves them for its gradient)
             made = attention.rope_tables(self._rotary.inv_freq.detach().to(device), self._positions, scale)
-        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
-            self._made[device] = made            # (a graph's hold nothing before its first replay: they stay its own)
+        if device.type == "cuda":
+            if torch.cuda.is_current_stream_capturing():
+                return made                      # (a graph's hold nothing before its first replay: they stay its own)
+            torch.cuda.current_stream(device).synchronize()
+        self._made[device] = made
         return made
 
 
@@ -399,7 +402,8 @@ def fuse_decoder_layers(model, enabled: bool = True, attention: bool = False) ->
     ``post_attention_layernorm`` and a ``ResidualDLRNet`` as ``mlp``).  With ``attention`` their attention modules also take the
     norms of queries and keys and the rotation as one kernel, forward and backward (modules of another form are left as
     they are; the rotation is in fp32, the host framework's in the model's type, and covers ``max_position_embeddings``
-    positions).  Returns how many layers were switched."""
+    positions; its tables are made here where the model is on a GPU, so that a capture of the first step holds none of that).
+    Returns how many layers were switched."""
     import types
     n = 0
     tables = RotaryTables(model) if enabled and attention and RotaryTables.fixed(model) else None
@@ -414,6 +418,8 @@ def fuse_decoder_layers(model, enabled: bool = True, attention: bool = False) ->
         if tables is not None and attention_fusable(attn):
             attn._rotary_tables = tables
             attn.forward = types.MethodType(_fused_attention_forward, attn)
+            if attn.q_proj.weight.is_cuda:
+                tables.on(attn.q_proj.weight.device)
         elif "_rotary_tables" in attn.__dict__:
             del attn.__dict__["_rotary_tables"]
             del attn.__dict__["forward"]
