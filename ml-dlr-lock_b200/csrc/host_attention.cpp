@@ -321,9 +321,9 @@ struct NormRope : torch::autograd::Function<NormRope> {
             Rows g[2], x[2] = {};
             at::Tensor kept[2];
             for (int i = 0; i < 2; ++i) {
-                kept[i] = grads[i];
+                kept[i] = grads[i].resolve_neg();
                 if (!rows_of(kept[i], &g[i])) {
-                    kept[i] = grads[i].clone(at::MemoryFormat::Contiguous);
+                    kept[i] = kept[i].clone(at::MemoryFormat::Contiguous);
                     TORCH_CHECK(rows_of(kept[i], &g[i]), "qk_norm_rope: gradients of unexpected shape");
                 }
             }

@@ -29,3 +29,15 @@ def test_forward_mode_derivatives_are_refused():
                 D.paged_attention(*args, table, n)
         D.qk_norm_rope(q, k, qw, kw, cos, sin, positions)          # (without a tangent all is as ever)
         D.paged_attention(row, kc, vc, table, n)
+
+
+def test_gradients_that_are_negated_lazily():
+    # (the imaginary part of a conjugate is such a tensor)
+    import dlr_lock_b200 as D
+    q, k, _, qw, kw, cos, sin, positions = _norm_rope_case(40, 4, 2, 64, 32, torch.float16, False, True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    out = D.qk_norm_rope(*leaves, cos, sin, positions)
+    grads = [_normal(_gen(i), *o.shape, dtype=o.dtype) for i, o in enumerate(out)]
+    want = torch.autograd.grad(out, leaves, [-g for g in grads], retain_graph=True)
+    got = torch.autograd.grad(out, leaves, [torch._neg_view(g) for g in grads])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
