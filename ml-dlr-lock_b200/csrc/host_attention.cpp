@@ -306,10 +306,39 @@ struct NormRope : torch::autograd::Function<NormRope> {
         return {out.first, out.second};
     }
 
+    // What was saved may have gone through hooks: other layouts are brought back, anything else is refused.
+    static void check_saved(int device, const at::Tensor (&grads)[2], at::Tensor* q, at::Tensor* k, at::Tensor* q_weight, at::Tensor* k_weight,
+                            at::Tensor* cos, at::Tensor* sin, at::Tensor* positions) {
+        const int64_t n = grads[0].dim(), dim = grads[0].size(n - 1);
+        const auto type = grads[0].scalar_type();
+        const auto back = [&](at::Tensor* t, bool as_given) {
+            TORCH_CHECK(t->is_cuda() && t->get_device() == device && t->layout() == at::kStrided && t->has_storage() && as_given,
+                        "qk_norm_rope: a saved tensor came back on another device, or with another type or shape");
+            *t = t->resolve_neg().contiguous();
+            if (!aligned(*t, 16)) *t = t->clone(at::MemoryFormat::Contiguous);
+        };
+        for (int i = 0; i < 2; ++i) {
+            at::Tensor *const x = i ? k : q, *const w = i ? k_weight : q_weight;
+            if (x->defined() && (!plain(*x, device) || x->scalar_type() != type || x->sizes() != grads[i].sizes() || !fits(*x)))
+                back(x, x->scalar_type() == type && x->sizes() == grads[i].sizes());
+            if (w->defined()) back(w, (w->scalar_type() == type || w->scalar_type() == at::kFloat) && w->dim() == 1 && w->size(0) == dim);
+        }
+        back(cos, cos->scalar_type() == at::kFloat && cos->dim() == 2 && cos->size(1) % 4 == 0 && 2 * cos->size(1) <= dim);
+        back(sin, sin->scalar_type() == at::kFloat && sin->sizes() == cos->sizes());
+        back(positions, (positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong) &&
+                            positions->sizes() == grads[0].sizes().slice(0, size_t(n - 2)));
+        TORCH_CHECK(!q_weight->defined() || !k_weight->defined() || q_weight->scalar_type() == k_weight->scalar_type(),
+                    "qk_norm_rope: the saved weights came back with two types");
+    }
+
+    static bool fits(const at::Tensor& t) {
+        Rows r;
+        return rows_of(t, &r);
+    }
+
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &q = saved[0], &k = saved[1], &q_weight = saved[2], &k_weight = saved[3], &cos = saved[4], &sin = saved[5],
-                         &positions = saved[6];
+        at::Tensor q = saved[0], k = saved[1], q_weight = saved[2], k_weight = saved[3], cos = saved[4], sin = saved[5], positions = saved[6];
         bool twice = false;
         torch::autograd::variable_list out(5);
         {
@@ -327,6 +356,7 @@ struct NormRope : torch::autograd::Function<NormRope> {
                     TORCH_CHECK(rows_of(kept[i], &g[i]), "qk_norm_rope: gradients of unexpected shape");
                 }
             }
+            check_saved(device, kept, &q, &k, &q_weight, &k_weight, &cos, &sin, &positions);
             if (q.defined()) TORCH_CHECK(rows_of(q, &x[0]), "qk_norm_rope: saved queries of unexpected layout");
             if (k.defined()) TORCH_CHECK(rows_of(k, &x[1]), "qk_norm_rope: saved keys of unexpected layout");
             for (int i = 0; i < 2; ++i) out[i] = at::empty(kept[i].sizes(), kept[i].options().memory_format(at::MemoryFormat::Contiguous));

@@ -41,3 +41,40 @@ def test_gradients_that_are_negated_lazily():
     want = torch.autograd.grad(out, leaves, [-g for g in grads], retain_graph=True)
     got = torch.autograd.grad(out, leaves, [torch._neg_view(g) for g in grads])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tensors_saved_through_hooks():
+    import dlr_lock_b200 as D
+    q, k, _, qw, kw, cos, sin, positions = _norm_rope_case(40, 4, 2, 64, 32, torch.bfloat16, False, True)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, qw, kw)]
+    grads = [_normal(_gen(i), *t.shape, dtype=t.dtype) for i, t in enumerate((q, k))]
+
+    def gradient(pack, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = D.qk_norm_rope(*leaves, cos, sin, positions)
+        return torch.autograd.grad(out, leaves, grads)
+
+    want = gradient(lambda t: t, lambda t: t)
+
+    def other_layout(t):
+        return torch.stack([t, t], -1)[..., 0] if t.dim() < 3 else t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    def off_boundary(t):
+        wide = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        wide[1:] = t.flatten()
+        return wide[1:].view(t.shape)
+
+    for pack, unpack in ((lambda t: t.cpu(), lambda t: t.to(DEV)), (lambda t: t, other_layout), (lambda t: t, off_boundary),
+                         (lambda t: -t, lambda t: torch._neg_view(t))):
+        assert all(torch.equal(a, b) for a, b in zip(gradient(pack, unpack), want))
+    # what comes back as something else is refused by the host
+    for unpack in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[:1], lambda t: t[None]):
+        for index in range(7):
+            seen = []
+
+            def once(t):
+                seen.append(t)
+                return unpack(t) if len(seen) == index + 1 else t
+
+            with pytest.raises(RuntimeError):
+                gradient(lambda t: t, once)
