@@ -246,7 +246,7 @@ struct Heads {
         half = cos.size(1);
         if (half % 4 || 2 * half > dim || cos.size(0) > kMostInt) return false;
         if ((positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) || positions.dim() != n - 2 ||
-            !same_leading(positions, q, n - 2) || !positions.is_contiguous())
+            !same_leading(positions, q, n - 2))
             return false;
         const at::Tensor* given[2] = {&q_weight, &k_weight};
         at::ScalarType type_of_weights = at::kFloat;
@@ -260,7 +260,13 @@ struct Heads {
             any = true;
         }
         weights_f32 = any && type_of_weights == at::kFloat;
-        return !wants_grad({&cos, &sin}) && !has_tangent({&q, &k, &q_weight, &k_weight, &cos, &sin});
+        if (wants_grad({&cos, &sin}) || has_tangent({&q, &k, &q_weight, &k_weight, &cos, &sin})) return false;
+        // (the host framework's positions are those of one row, expanded over the batch)
+        if (!positions.is_contiguous()) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            positions = positions.contiguous();
+        }
+        return true;
     }
 
     dlrb200_norm_rope_args args() const {

@@ -78,3 +78,25 @@ def test_tensors_saved_through_hooks():
 
             with pytest.raises(RuntimeError):
                 gradient(lambda t: t, once)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_positions_of_one_row_for_a_batch_are_taken_as_they_are(kind):
+    # what the host framework gives its layers: one row, expanded; taken by the native side, not checked and copied in Python first
+    import dlr_lock_b200 as D
+    from dlr_lock_b200 import attention
+    q, k, v, qw, kw, cos, sin, _ = _norm_rope_case(3 * 50, 4, 2, 64, 32, torch.bfloat16, False, True)
+    q, k, v = (t.unflatten(0, (3, 50)) for t in (q, k, v))
+    row = torch.arange(7, 57, device=DEV, dtype=kind)[None]
+    want = D.qk_norm_rope(q, k, qw, kw, cos, sin, row.repeat(3, 1))
+    native = attention._native()
+    got = native.qk_norm_rope(q, k, qw, kw, cos, sin, row.expand(3, 50), 1e-6, False)
+    assert type(got) is tuple and all(torch.equal(a, b) for a, b in zip(got, want))
+    slots = torch.arange(150, device=DEV, dtype=torch.int32).view(3, 50)
+    kc, vc = torch.zeros(2, 10, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    got = native.qk_norm_rope_append(q, k, qw, kw, cos, sin, row.expand(3, 50), v, slots, kc, vc, 1e-6, False, False)
+    assert torch.equal(got, want[0]) and torch.equal(kc.transpose(1, 2).flatten(0, 1)[:150], want[1].flatten(0, 1))
+    leaves = [t.detach().requires_grad_(True) for t in (q, k)]
+    grads = [_normal(_gen(i), *t.shape, dtype=t.dtype) for i, t in enumerate(leaves)]
+    both = [torch.autograd.grad(D.qk_norm_rope(*leaves, qw, kw, cos, sin, p), leaves, grads) for p in (row.expand(3, 50), row.repeat(3, 1))]
+    assert all(torch.equal(a, b) for a, b in zip(*both))
