@@ -122,6 +122,13 @@ bool real(PyObject* o, double* v) {
     return true;
 }
 
+// The truth of a flag; false with Python's error set where it has none.
+bool flag(PyObject* o, bool* v) {
+    const int is = PyObject_IsTrue(o);
+    *v = is == 1;
+    return is >= 0;
+}
+
 // (a dimension of one has any stride)
 int64_t step_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.stride(i); }
 
@@ -130,6 +137,8 @@ int64_t step_of(const at::Tensor& t, int64_t i) { return t.size(i) == 1 ? 0 : t.
 PyObject* paged_plan(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     if (n_args != 10) Py_RETURN_NONE;
+    bool in_place;
+    if (!flag(o[9], &in_place)) return nullptr;
     const at::Tensor *lengths = tensor(o[0]), *fresh = tensor(o[1]), *table = tensor(o[2]), *pages = tensor(o[3]), *count = tensor(o[4]);
     const at::Tensor* finished = o[8] == Py_None ? nullptr : tensor(o[8]);
     if (!lengths || !fresh || !table || !pages || !count || (o[8] != Py_None && !finished)) Py_RETURN_NONE;
@@ -169,7 +178,6 @@ PyObject* paged_plan(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
         slots = part(0, rows);
         positions = part(rows, rows);
         starts = part(2 * rows, n + 1);
-        const bool in_place = PyObject_IsTrue(o[9]) == 1;
         lengths_out = in_place ? *lengths : part(2 * rows + n + 1, n);
         count_out = in_place ? *count : part(2 * rows + 2 * n + 1, 1);
     }
@@ -426,7 +434,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
     Heads h;
     if (n_args != 9 || !heads_from(o, &h) || !real(o[7], &h.eps)) Py_RETURN_NONE;
-    h.interleaved = PyObject_IsTrue(o[8]) == 1;
+    if (!flag(o[8], &h.interleaved)) return nullptr;
     if (!h.check()) Py_RETURN_NONE;
     if (!wants_grad({&h.q, &h.k, &h.q_weight, &h.k_weight})) {
         auto out = turned(h);
@@ -460,7 +468,8 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n_args) 
     if (n_args != 14 || !heads_from(o, &h) || !real(o[11], &h.eps)) Py_RETURN_NONE;
     const at::Tensor *v = tensor(o[7]), *slots = tensor(o[8]), *k_cache = tensor(o[9]), *v_cache = tensor(o[10]);
     if (!v || !slots || !k_cache || !v_cache) Py_RETURN_NONE;
-    h.interleaved = PyObject_IsTrue(o[12]) == 1;
+    bool keys;
+    if (!flag(o[12], &h.interleaved) || !flag(o[13], &keys)) return nullptr;
     if (!h.check() || wants_grad({&h.q, &h.k, v, &h.q_weight, &h.k_weight, k_cache, v_cache}) || has_tangent({v, k_cache, v_cache})) Py_RETURN_NONE;
     Rows v_rows;
     Cache kc, vc;
@@ -470,7 +479,6 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n_args) 
     if (!cache_of(*k_cache, h.device, h.q.scalar_type(), kv_heads, h.dim, 4, &kc) || !cache_of(*v_cache, h.device, h.q.scalar_type(), kv_heads, h.dim, 4, &vc) ||
         k_cache->sizes() != v_cache->sizes())
         Py_RETURN_NONE;
-    const bool keys = PyObject_IsTrue(o[13]) == 1;
     at::Tensor q_out, k_out;
     {
         at::AutoDispatchBelowADInplaceOrView below;

@@ -4,7 +4,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import dlr_lock_b200 as D
-from test_attention_refusals import _append_args, _attention_args, _heads_args
+from test_attention_refusals import _append_args, _attention_args, _heads_args, _plan_args
 
 
 @pytest.mark.parametrize("call,args,names", [
@@ -23,3 +23,19 @@ def test_forward_mode_derivatives_are_refused(call, args, names, grad):
                 call(**given)
         with pytest.raises(ValueError, match="CUDA"):              # (no tangent: the next check)
             call(**args())
+
+
+class _NoTruth:
+    def __bool__(self):
+        raise ValueError("neither true nor false")
+
+
+@pytest.mark.parametrize("call,args,name", [
+    (D.qk_norm_rope, _heads_args, "interleaved"),
+    (D.qk_norm_rope_append, _append_args, "interleaved"),
+    (D.qk_norm_rope_append, _append_args, "return_keys"),
+    (D.paged_plan, _plan_args, "in_place"),
+])
+def test_a_flag_without_a_truth_value_raises_its_own_error(call, args, name):
+    with torch.no_grad(), pytest.raises(ValueError, match="neither true nor false"):
+        call(**args(), **{name: _NoTruth()})
