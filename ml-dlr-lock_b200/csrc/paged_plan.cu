@@ -13,6 +13,7 @@
 
 #include <limits.h>
 
+#include "dlr_b200.h"
 #include "ptx.cuh"
 
 namespace dlr {
@@ -222,8 +223,10 @@ cudaError_t paged_plan(const PlanArgs& a, int smem_optin, cudaStream_t stream) {
     const size_t smem = size_t(a.requests) * 4 * sizeof(int);
     auto kern = cluster ? plan_kernel<true> : plan_kernel<false>;
     if (smem > 40 * 1024) {
-        if (smem + 1024 > size_t(smem_optin)) return cudaErrorInvalidValue;
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        // the most that any call takes: a call of fewer requests in another thread, between this and the launch, would lower it
+        constexpr int kMost = DLRB200_MAX_PLAN_REQUESTS * 4 * int(sizeof(int));
+        if (smem > size_t(kMost) || kMost + 1024 > smem_optin) return cudaErrorInvalidValue;
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchAttribute attr[1];

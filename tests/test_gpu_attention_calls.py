@@ -100,3 +100,33 @@ def test_positions_of_one_row_for_a_batch_are_taken_as_they_are(kind):
     grads = [_normal(_gen(i), *t.shape, dtype=t.dtype) for i, t in enumerate(leaves)]
     both = [torch.autograd.grad(D.qk_norm_rope(*leaves, qw, kw, cos, sin, p), leaves, grads) for p in (row.expand(3, 50), row.repeat(3, 1))]
     assert all(torch.equal(a, b) for a, b in zip(*both))
+
+
+def test_plans_of_many_requests_from_two_threads():
+    # through the C ABI, which a host calls without Python's lock
+    import ctypes
+    import threading
+    from dlr_lock_b200 import _lib
+    lib = _lib.load()
+    refused = {}
+
+    def plans(requests):
+        def zeros(*shape):
+            return torch.zeros(*shape, dtype=torch.int32, device=DEV)
+
+        t = dict(lengths=zeros(requests), new_tokens=zeros(requests), block_table=zeros(requests, 1), free_pages=zeros(8), n_free=zeros(1),
+                 slots=zeros(requests), positions=zeros(requests), starts=zeros(requests + 1), lengths_out=zeros(requests), n_free_out=zeros(1))
+        step = _lib.PlanStep(**{n: x.data_ptr() for n, x in t.items()}, table_stride=1, requests=requests, columns=1, pages=8, page_size=16,
+                             width=1, rows=requests)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        refused[requests] = sum(lib.dlrb200_paged_plan(ctypes.byref(step), ctypes.c_void_p(stream.cuda_stream)) != 0 for _ in range(4000))
+        stream.synchronize()
+        assert t["starts"].tolist() == list(range(requests + 1))
+
+    threads = [threading.Thread(target=plans, args=(n,)) for n in (8192, 2600, 700)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert refused == {8192: 0, 2600: 0, 700: 0}
