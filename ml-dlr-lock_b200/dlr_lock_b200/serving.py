@@ -36,13 +36,14 @@ class PagedCache:
         if pages < 1 or pages * page_size > 0x7fffffff or requests > attention.MAX_REQUESTS:
             raise ValueError(f"PagedCache: {pages} pages of {page_size} for {requests} requests")
         self.page_size, self.max_tokens = page_size, columns * page_size
-        # (what no token was written to is never read: the memory is not cleared)
-        self.values = torch.empty(layers, 2, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device)
         ints = dict(dtype=torch.int32, device=device)
-        self.block_table = torch.full((requests, columns), -1, **ints)
-        self.lengths = torch.zeros(requests, **ints)
-        self.free_pages = torch.arange(pages - 1, -1, -1, **ints)
-        self.n_free = torch.full((1,), pages, **ints)
+        with torch.inference_mode(False):        # (a cache made in inference mode may be written to outside of it)
+            # (what no token was written to is never read: the memory is not cleared)
+            self.values = torch.empty(layers, 2, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device)
+            self.block_table = torch.full((requests, columns), -1, **ints)
+            self.lengths = torch.zeros(requests, **ints)
+            self.free_pages = torch.arange(pages - 1, -1, -1, **ints)
+            self.n_free = torch.full((1,), pages, **ints)
 
     @property
     def requests(self) -> int:
