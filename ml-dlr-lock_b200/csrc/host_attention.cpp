@@ -461,6 +461,13 @@ bool cache_of(const at::Tensor& t, int device, at::ScalarType type, int64_t head
                               aligned(t, uintptr_t(2 * multiple)));
 }
 
+// An expanded cache, of which slots lie in one place: nothing to write to.
+bool expanded(const at::Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1 && t.stride(i) == 0) return t.numel() > 0;
+    return false;
+}
+
 // (q, k, q_weight, k_weight, cos, sin, positions, v, slots, k_cache, v_cache, eps, interleaved, return_keys)
 PyObject* qk_norm_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n_args) {
     HANDLE_TH_ERRORS
@@ -477,7 +484,7 @@ PyObject* qk_norm_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n_args) 
     if (!plain(*v, h.device) || v->scalar_type() != h.k.scalar_type() || v->sizes() != h.k.sizes() || !rows_of(*v, &v_rows)) Py_RETURN_NONE;
     if (!ints(*slots, h.device) || slots->dim() != n - 2 || !same_leading(*slots, h.q, n - 2)) Py_RETURN_NONE;
     if (!cache_of(*k_cache, h.device, h.q.scalar_type(), kv_heads, h.dim, 4, &kc) || !cache_of(*v_cache, h.device, h.q.scalar_type(), kv_heads, h.dim, 4, &vc) ||
-        k_cache->sizes() != v_cache->sizes())
+        k_cache->sizes() != v_cache->sizes() || expanded(*k_cache) || expanded(*v_cache))
         Py_RETURN_NONE;
     at::Tensor q_out, k_out;
     {

@@ -39,3 +39,11 @@ class _NoTruth:
 def test_a_flag_without_a_truth_value_raises_its_own_error(call, args, name):
     with torch.no_grad(), pytest.raises(ValueError, match="neither true nor false"):
         call(**args(), **{name: _NoTruth()})
+
+
+@pytest.mark.parametrize("name", ["k_cache", "v_cache"])
+@pytest.mark.parametrize("shape", [(1, 2, 16, 64), (3, 1, 16, 64), (3, 2, 1, 64)])
+def test_append_refuses_caches_of_which_slots_share_memory(name, shape):
+    shared = torch.zeros(shape, dtype=torch.bfloat16).expand(3, 2, 16, 64)
+    with torch.no_grad(), pytest.raises(ValueError, match="share memory"):
+        D.qk_norm_rope_append(**_append_args(**{name: shared}))

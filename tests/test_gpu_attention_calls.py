@@ -130,3 +130,17 @@ def test_plans_of_many_requests_from_two_threads():
     for t in threads:
         t.join()
     assert refused == {8192: 0, 2600: 0, 700: 0}
+
+
+def test_append_refuses_caches_of_which_slots_share_memory():
+    import dlr_lock_b200 as D
+    q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(9, 4, 2, 64, 32, torch.bfloat16, False, True)
+    slots = torch.arange(9, dtype=torch.int32, device=DEV)
+    whole = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    for shape in ((1, 2, 16, 64), (3, 1, 16, 64), (3, 2, 1, 64)):
+        shared = torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+        for caches in ((shared.expand(3, 2, 16, 64), whole), (whole, shared.expand(3, 2, 16, 64))):
+            with pytest.raises(ValueError, match="share memory"):
+                D.qk_norm_rope_append(q, k, v, qw, kw, cos, sin, positions, slots, *caches)
+        assert not shared.any()
+    assert not whole.any()
