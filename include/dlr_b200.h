@@ -226,7 +226,7 @@ typedef struct dlrb200_plan_step {
     const int* lengths;             /* (requests) tokens held */
     const int* new_tokens;          /* (requests) */
     const unsigned char* finished;  /* (requests) or null */
-    int* block_table;               /* (requests, columns), rows table_stride elements apart */
+    int* block_table;               /* (requests, columns), rows table_stride elements apart (columns at least) */
     int64_t table_stride;
     int* free_pages;                /* (pages) */
     const int* n_free;              /* (1) */

@@ -762,6 +762,7 @@ int dlrb200_paged_plan(const dlrb200_plan_step* s, void* stream) {
     if (!s->n_free || !s->starts || !s->n_free_out || (s->rows > 0 && (!s->slots || !s->positions)) || (s->pages > 0 && !s->free_pages) ||
         (s->requests > 0 && (!s->lengths || !s->new_tokens || !s->lengths_out || (s->columns > 0 && !s->block_table))))
         return DLRB200_ERR_INVALID_ARG;
+    if (s->requests > 1 && s->table_stride < s->columns) return DLRB200_ERR_INVALID_ARG;      // (the rows are written)
     DevInfo di;
     const int rc = device_b200(&di);
     if (rc != DLRB200_OK) return rc;

@@ -47,3 +47,17 @@ def test_append_refuses_caches_of_which_slots_share_memory(name, shape):
     shared = torch.zeros(shape, dtype=torch.bfloat16).expand(3, 2, 16, 64)
     with torch.no_grad(), pytest.raises(ValueError, match="share memory"):
         D.qk_norm_rope_append(**_append_args(**{name: shared}))
+
+
+def test_the_c_abi_refuses_tables_whose_rows_overlap():
+    import ctypes
+    from dlr_lock_b200 import _lib
+    from dlr_lock_b200.build import build_library
+    build_library()
+    lib = _lib.load()
+    word = (ctypes.c_int * 64)()
+    at = ctypes.cast(word, ctypes.c_void_p).value & ~63
+    plan = dict(lengths=at, new_tokens=at, block_table=at, free_pages=at, n_free=at, slots=at, positions=at, starts=at, lengths_out=at,
+                n_free_out=at, requests=2, columns=4, pages=8, page_size=16, width=1, rows=2)
+    for stride in (0, 3, -4):
+        assert lib.dlrb200_paged_plan(ctypes.byref(_lib.PlanStep(**plan, table_stride=stride)), None) == 1
