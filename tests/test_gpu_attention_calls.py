@@ -144,3 +144,37 @@ def test_append_refuses_caches_of_which_slots_share_memory():
                 D.qk_norm_rope_append(q, k, v, qw, kw, cos, sin, positions, slots, *caches)
         assert not shared.any()
     assert not whole.any()
+
+
+@pytest.mark.parametrize("kind", ["expanded", "transposed", "strided", "as they are"])
+def test_incoming_gradients_of_any_layout(kind):
+    # four dimensions, no query norm, int32 positions; an expanded gradient has stride 0, others are read where they lie or copied
+    import dlr_lock_b200 as D
+    q, k, _, qw, kw, cos, sin, positions = _norm_rope_case(300, 16, 8, 128, 64, torch.bfloat16, False, True)
+    leaves = [q.view(3, 100, 16, 128).detach().requires_grad_(True), k.view(3, 100, 8, 128).detach().requires_grad_(True),
+              kw.detach().requires_grad_(True)]
+    where = positions.view(3, 100).int()
+    out = D.qk_norm_rope(leaves[0], leaves[1], None, leaves[2], cos, sin, where)
+    grads = [_normal(_gen(i), *o.shape, dtype=o.dtype) for i, o in enumerate(out)]
+    if kind == "expanded":
+        grads = [torch.ones((), dtype=g.dtype, device=DEV).expand(g.shape) for g in grads]
+    elif kind == "transposed":
+        grads = [g.transpose(1, 2).contiguous().transpose(1, 2) for g in grads]
+    elif kind == "strided":
+        grads = [torch.stack([g, g], 3)[:, :, :, 0] for g in grads]
+    got = torch.autograd.grad(out, leaves, grads)
+    # 64 bits
+    exact = [t.detach().double().requires_grad_(True) for t in leaves]
+    c, s = cos[where.long()][:, :, None].double(), sin[where.long()][:, :, None].double()
+    x = exact[1] * (exact[1].square().mean(-1, keepdim=True) + 1e-6).rsqrt() * exact[2]
+    turned = []
+    for t in (exact[0], x):
+        a, b = t.chunk(2, -1)
+        turned.append(torch.cat([a * c - b * s, b * c + a * s], -1))
+    want = torch.autograd.grad(turned, exact, [g.double() for g in grads])
+    for mine, its in zip(got, want):
+        # rounded once; fp32 before: 128 products in each sum of a head, 2400 heads in that of the weight, half-steps of 2^-24 of the
+        # sizes summed, which are below 16 times (a head) and 2400 x 16 (the weight) a gradient of 1 to 5
+        sums = 2400 * 16 * 5 if its.dim() == 1 else 128 * 16 * 5
+        bound = torch.finfo(mine.dtype).eps / 2 * its.abs() + sums * 2.0 ** -24
+        assert ((mine.double() - its).abs() <= bound).all()
