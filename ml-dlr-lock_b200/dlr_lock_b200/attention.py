@@ -285,7 +285,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     _check_cache(what, k_cache, v_cache, q.dtype, k.shape[-2], dim, 4)
     if any(n > 1 and not step for c in (k_cache, v_cache) if c.numel() for n, step in zip(c.shape, c.stride())):
         raise ValueError(f"{what}: slots of the caches share memory")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight, k_cache, v_cache)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
     _no_tangents(what, q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)
     device = _on_one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache)

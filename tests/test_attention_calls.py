@@ -61,3 +61,11 @@ def test_the_c_abi_refuses_tables_whose_rows_overlap():
                 n_free_out=at, requests=2, columns=4, pages=8, page_size=16, width=1, rows=2)
     for stride in (0, 3, -4):
         assert lib.dlrb200_paged_plan(ctypes.byref(_lib.PlanStep(**plan, table_stride=stride)), None) == 1
+
+
+@pytest.mark.parametrize("name", ["cos", "sin"])
+def test_append_names_tables_that_want_a_gradient(name):
+    given = _append_args()
+    given[name].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        D.qk_norm_rope_append(**given)
