@@ -86,6 +86,12 @@ def _no_tangents(what, *tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
+def _not_negated(what, *tensors):
+    for t in tensors:
+        if t is not None and t.is_neg():
+            raise ValueError(f"{what}: tensors that are negated lazily are not taken here")
+
+
 def _int32(what, name, t, shape):
     if t.dtype != torch.int32:
         raise TypeError(f"{what}: {name} has type {t.dtype}, expected int32")
@@ -109,6 +115,7 @@ def _check_cache(what, k_cache, v_cache, dtype, kv_heads, dim, multiple):
         raise TypeError(f"{what}: the caches have types {k_cache.dtype} and {v_cache.dtype}, expected {dtype}")
     if k_cache.shape[1] != kv_heads or k_cache.shape[3] != dim:
         raise ValueError(f"{what}: the caches have shape {tuple(k_cache.shape)}, expected {kv_heads} heads of {dim}")
+    _not_negated(what, k_cache, v_cache)
     _page_size(what, k_cache.shape[2])
     if k_cache.shape[0] * k_cache.shape[2] > 0x7fffffff:
         raise ValueError(f"{what}: the caches have more than 2^31 - 1 slots")
@@ -120,6 +127,7 @@ def _check_cache(what, k_cache, v_cache, dtype, kv_heads, dim, multiple):
 
 def _heads(t: torch.Tensor, multiple: int) -> torch.Tensor:
     """t if its rows can be read where they are, else a contiguous copy."""
+    t = t.resolve_neg()
     one = t.dim() <= 3 or t.is_contiguous()               # the leading dimensions are a single one
     if one and t.stride(-1) == 1 and not any(s % multiple for s in t.stride()[:-1]) and t.data_ptr() % (2 * multiple) == 0:
         return t
@@ -176,6 +184,7 @@ def paged_plan(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
         rows = width * n
     if type(rows) is not int or rows < 0 or rows > 1 << 30:
         raise ValueError(f"{what}: {rows} rows, 0 to 2^30 are possible")
+    _not_negated(what, lengths, new_tokens, block_table, free_pages, n_free, finished)
     device = _on_one_device(what, lengths, new_tokens, block_table, free_pages, n_free, finished)
     with torch.cuda.device(device):
         out = _native().paged_plan(lengths, new_tokens, block_table, free_pages, n_free, page_size, width, rows, finished, in_place)
@@ -226,6 +235,7 @@ def _check_norm_rope(what, q, k, q_weight, k_weight, cos, sin, positions):
 
 def _vector(w):
     """A weight as the kernels read it: contiguous from a 16-byte boundary."""
+    w = w if w is None else w.resolve_neg()
     if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0):
         return w
     return w.clone(memory_format=torch.contiguous_format)
@@ -233,7 +243,8 @@ def _vector(w):
 
 def _in_shape(q, k, q_weight, k_weight, cos, sin, positions):
     """The arguments laid out as the kernels read them; gradients pass through."""
-    return _heads(q, 4), _heads(k, 4), _vector(q_weight), _vector(k_weight), cos, sin, positions.contiguous()
+    return (_heads(q, 4), _heads(k, 4), _vector(q_weight), _vector(k_weight), cos.resolve_neg(), sin.resolve_neg(),
+            positions.resolve_neg().contiguous())
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -285,13 +296,15 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     _check_cache(what, k_cache, v_cache, q.dtype, k.shape[-2], dim, 4)
     if any(n > 1 and not step for c in (k_cache, v_cache) if c.numel() for n, step in zip(c.shape, c.stride())):
         raise ValueError(f"{what}: slots of the caches share memory")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)):
+    given = (q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-    _no_tangents(what, q, k, v, q_weight, k_weight, cos, sin, k_cache, v_cache)
+    _no_tangents(what, *given)
     device = _on_one_device(what, q, k, v, q_weight, k_weight, cos, sin, positions, slots, k_cache, v_cache)
     with torch.cuda.device(device):
-        out = _native().qk_norm_rope_append(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), _heads(v, 4), slots.contiguous(),
-                                            k_cache, v_cache, float(eps), bool(interleaved), bool(return_keys))
+        out = _native().qk_norm_rope_append(*_in_shape(q, k, q_weight, k_weight, cos, sin, positions), _heads(v, 4),
+                                            slots.resolve_neg().contiguous(), k_cache, v_cache, float(eps), bool(interleaved),
+                                            bool(return_keys))
     return _result(out, "dlrb200_qk_norm_rope")
 
 
@@ -334,5 +347,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _no_tangents(what, q, k_cache, v_cache)
     device = _on_one_device(what, q, k_cache, v_cache, block_table, lengths)
     with torch.cuda.device(device):
-        out = _native().paged_attention(_heads(q, 2), k_cache, v_cache, block_table, lengths, None if scale is None else float(scale))
+        out = _native().paged_attention(_heads(q, 2), k_cache, v_cache, block_table.resolve_neg(), lengths.resolve_neg(),
+                                        None if scale is None else float(scale))
     return _result(out, "dlrb200_paged_attention")

@@ -178,3 +178,32 @@ def test_incoming_gradients_of_any_layout(kind):
         sums = 2400 * 16 * 5 if its.dim() == 1 else 128 * 16 * 5
         bound = torch.finfo(mine.dtype).eps / 2 * its.abs() + sums * 2.0 ** -24
         assert ((mine.double() - its).abs() <= bound).all()
+
+
+def test_inputs_that_are_negated_lazily():
+    import dlr_lock_b200 as D
+    q, k, v, qw, kw, cos, sin, positions = _norm_rope_case(40, 4, 2, 64, 32, torch.float16, False, True)
+
+    def lazy(t):
+        return torch._neg_view(-t)
+
+    want = D.qk_norm_rope(q, k, qw, kw, cos, sin, positions)
+    got = D.qk_norm_rope(lazy(q), lazy(k), lazy(qw), lazy(kw), lazy(cos), lazy(sin), lazy(positions))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    slots = torch.arange(40, dtype=torch.int32, device=DEV)
+    caches = [torch.zeros(2, 3, 2, 16, 64, dtype=torch.float16, device=DEV) for _ in range(2)]
+    D.qk_norm_rope_append(q, k, v, qw, kw, cos, sin, positions, slots, *caches[0])
+    D.qk_norm_rope_append(q, k, lazy(v), qw, kw, cos, sin, positions, lazy(slots), *caches[1])
+    assert torch.equal(*caches)
+    kc, vc, table, n = _cache_case([40], 2, 64, 32, torch.float16)
+    row = _normal(_gen(0), 1, 4, 64, dtype=torch.float16)
+    want = D.paged_attention(row, kc, vc, table, n)
+    assert torch.equal(D.paged_attention(lazy(row), kc, vc, lazy(table), lazy(n)), want)
+    # what would be written to is refused
+    with pytest.raises(ValueError, match="negated"):
+        D.qk_norm_rope_append(q, k, v, qw, kw, cos, sin, positions, slots, torch._neg_view(caches[0][0]), caches[0][1])
+    with pytest.raises(ValueError, match="negated"):
+        D.paged_attention(row, torch._neg_view(kc), vc, table, n)
+    free, count = torch.arange(4, dtype=torch.int32, device=DEV), torch.tensor([4], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="negated"):
+        D.paged_plan(n, torch._neg_view(n), table, free, count, 32)
