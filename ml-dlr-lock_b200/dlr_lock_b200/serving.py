@@ -104,6 +104,11 @@ class PagedDecoder:
             h = layer.mlp.dlrnet(h + attn.o_proj(out.flatten(1)))
         return h
 
+    def _flags(self, what, name, flags):
+        if flags.shape != (self.cache.requests,):
+            raise ValueError(f"{what}: {name} must have shape {(self.cache.requests,)}, not {tuple(flags.shape)}")
+        return flags.bool()
+
     def _embed(self, ids, plan):
         """Embeddings of the rows that have a token; what stands in the others' ids is not looked up."""
         return self.model.model.embed_tokens(ids.flatten().masked_fill(plan.slots < 0, 0))
@@ -123,7 +128,7 @@ class PagedDecoder:
         if counts.dtype != torch.int32 or counts.shape != (cache.requests,):
             raise ValueError(f"admit: counts must be int32 of shape {(cache.requests,)}")
         width = ids.shape[1]
-        again = counts > 0 if finished is None else (counts > 0) | finished
+        again = counts > 0 if finished is None else (counts > 0) | self._flags("admit", "finished", finished)
         plan = cache.plan(counts, width, again)
 
         def attend(attn, q, k, v, where, eps):
@@ -145,7 +150,7 @@ class PagedDecoder:
         cache = self.cache
         if tokens.shape != (cache.requests,):
             raise ValueError(f"step: expected tokens ({cache.requests},), got {tuple(tokens.shape)}")
-        plan = cache.plan(self._one if active is None else active.to(torch.int32))
+        plan = cache.plan(self._one if active is None else self._flags("step", "active", active).to(torch.int32))
 
         def attend(attn, q, k, v, where, eps):
             q = attention.qk_norm_rope_append(q, k, v, *where, eps=eps)
