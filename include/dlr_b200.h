@@ -207,7 +207,8 @@ DLRB200_API int dlrb200_forward_static(const void* x, void* y, const void* Vp, c
  * There is no counterpart in the reference, whose decode loop leaves attention
  * and cache to the host framework (dlr_lock/model.py:156-176 replaces only the
  * MLP of a layer).  Like all calls of this library these are asynchronous on
- * `stream`, allocate nothing and can be captured in a CUDA graph.
+ * `stream`, allocate nothing and can be captured in a CUDA graph.  Integers lie
+ * on their natural boundaries.
  * ------------------------------------------------------------------------- */
 #define DLRB200_BF16 0
 #define DLRB200_F16 1

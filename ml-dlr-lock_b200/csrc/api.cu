@@ -763,6 +763,9 @@ int dlrb200_paged_plan(const dlrb200_plan_step* s, void* stream) {
         (s->requests > 0 && (!s->lengths || !s->new_tokens || !s->lengths_out || (s->columns > 0 && !s->block_table))))
         return DLRB200_ERR_INVALID_ARG;
     if (s->requests > 1 && s->table_stride < s->columns) return DLRB200_ERR_INVALID_ARG;      // (the rows are written)
+    for (const int* p : std::initializer_list<const int*>{s->lengths, s->new_tokens, s->block_table, s->free_pages, s->n_free, s->slots, s->positions,
+                                                          s->starts, s->lengths_out, s->n_free_out})
+        if (!aligned(p, 4)) return DLRB200_ERR_ALIGNMENT;
     DevInfo di;
     const int rc = device_b200(&di);
     if (rc != DLRB200_OK) return rc;
@@ -788,7 +791,8 @@ int dlrb200_qk_norm_rope(const dlrb200_norm_rope_args* s, void* stream) {
     if (!cache && !s->k_out) return DLRB200_ERR_INVALID_ARG;
     if (cache && (!s->v || (s->pages > 0 && (!s->k_cache || !s->v_cache)))) return DLRB200_ERR_INVALID_ARG;
     if (!multiples(4, {s->q_token, s->q_head, s->k_token, s->k_head}) || !aligned(s->q, 8) || !aligned(s->k, 8) || !aligned(s->q_out, 8) ||
-        !aligned(s->k_out, 8) || !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16))
+        !aligned(s->k_out, 8) || !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16) ||
+        !aligned(s->positions, s->positions_64 ? 8 : 4) || !aligned(s->slots, 4))
         return DLRB200_ERR_ALIGNMENT;
     if (cache && (!multiples(4, {s->v_token, s->v_head, s->kc_page, s->kc_head, s->kc_slot, s->vc_page, s->vc_head, s->vc_slot}) ||
                   !aligned(s->v, 8) || !aligned(s->k_cache, 8) || !aligned(s->v_cache, 8)))
@@ -827,7 +831,9 @@ int dlrb200_qk_norm_rope_backward(const dlrb200_norm_rope_grad_args* s, void* st
         return DLRB200_ERR_INVALID_ARG;
     if (!multiples(4, {s->q_token, s->q_head, s->k_token, s->k_head, s->qg_token, s->qg_head, s->kg_token, s->kg_head}) || !aligned(s->q, 8) ||
         !aligned(s->k, 8) || !aligned(s->q_grad, 8) || !aligned(s->k_grad, 8) || !aligned(s->dq, 8) || !aligned(s->dk, 8) ||
-        !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16))
+        !aligned(s->cos, 16) || !aligned(s->sin, 16) || !aligned(s->q_weight, 16) || !aligned(s->k_weight, 16) ||
+        !aligned(s->positions, s->positions_64 ? 8 : 4) || !aligned(s->dq_weight, s->weights_f32 ? 4 : 2) ||
+        !aligned(s->dk_weight, s->weights_f32 ? 4 : 2))
         return DLRB200_ERR_ALIGNMENT;
     if (weights && (!s->workspace || s->workspace_bytes < dlrb200_qk_norm_rope_backward_workspace_bytes(s->dim))) return DLRB200_ERR_WORKSPACE;
     if (weights && !aligned(s->workspace, 16)) return DLRB200_ERR_ALIGNMENT;
@@ -862,7 +868,8 @@ int dlrb200_paged_attention(const dlrb200_paged_attention_args* s, void* stream)
     if (!s->q || !s->lengths || !s->out || (s->pages > 0 && (!s->k_cache || !s->v_cache)) || (s->columns > 0 && !s->block_table))
         return DLRB200_ERR_INVALID_ARG;
     if (!multiples(2, {s->q_request, s->q_head}) || !multiples(8, {s->kc_page, s->kc_head, s->kc_slot, s->vc_page, s->vc_head, s->vc_slot}) ||
-        !aligned(s->q, 4) || !aligned(s->k_cache, 16) || !aligned(s->v_cache, 16) || !aligned(s->out, 16) || !aligned(s->workspace, 16))
+        !aligned(s->q, 4) || !aligned(s->k_cache, 16) || !aligned(s->v_cache, 16) || !aligned(s->out, 16) || !aligned(s->workspace, 16) ||
+        !aligned(s->block_table, 4) || !aligned(s->lengths, 4))
         return DLRB200_ERR_ALIGNMENT;
     if (!s->workspace || s->workspace_bytes < dlrb200_paged_attention_workspace_bytes(s->heads, s->kv_heads, s->dim)) return DLRB200_ERR_WORKSPACE;
     DevInfo di;

@@ -69,3 +69,31 @@ def test_append_names_tables_that_want_a_gradient(name):
     given[name].requires_grad_(True)
     with pytest.raises(RuntimeError, match="has no gradient"):
         D.qk_norm_rope_append(**given)
+
+
+def test_the_c_abi_refuses_integers_off_their_boundaries():
+    import ctypes
+    from dlr_lock_b200 import _lib
+    from dlr_lock_b200.build import build_library
+    build_library()
+    lib, ref = _lib.load(), ctypes.byref
+    word = (ctypes.c_int * 64)()
+    at = ctypes.cast(word, ctypes.c_void_p).value & ~63
+    plan = dict(lengths=at, new_tokens=at, block_table=at, table_stride=4, free_pages=at, n_free=at, slots=at, positions=at, starts=at,
+                lengths_out=at, n_free_out=at, requests=2, columns=4, pages=8, page_size=16, width=1, rows=2)
+    for name in [n for n, v in plan.items() if v == at]:
+        assert lib.dlrb200_paged_plan(ref(_lib.PlanStep(**{**plan, name: at + 2})), None) == 3, name
+    heads = dict(cos=at, sin=at, positions=at, tokens=1, q_heads=1, k_heads=1, dim=64, half=32, table_rows=1)
+    norm = dict(heads, q=at, k=at, v=at, q_out=at, k_out=at, slots=at, k_cache=at, v_cache=at, pages=1, page_size=16)
+    grad = dict(heads, q=at, k=at, q_grad=at, k_grad=at, dq=at, dk=at)
+    for changed in (dict(positions=at + 2), dict(positions=at + 4, positions_64=1), dict(positions_64=1, positions=at + 1)):
+        assert lib.dlrb200_qk_norm_rope(ref(_lib.NormRopeArgs(**{**norm, **changed})), None) == 3, changed
+        assert lib.dlrb200_qk_norm_rope_backward(ref(_lib.NormRopeGradArgs(**{**grad, **changed})), None) == 3, changed
+    assert lib.dlrb200_qk_norm_rope(ref(_lib.NormRopeArgs(**{**norm, "slots": at + 2})), None) == 3
+    for changed in (dict(dq_weight=at + 1), dict(dk_weight=at + 1), dict(dk_weight=at + 2, weights_f32=1)):
+        weights = dict(q_weight=at, k_weight=at, workspace=at, workspace_bytes=1 << 40)
+        assert lib.dlrb200_qk_norm_rope_backward(ref(_lib.NormRopeGradArgs(**{**grad, **weights, **changed})), None) == 3, changed
+    attend = dict(q=at, q_request=64, q_head=64, k_cache=at, v_cache=at, block_table=at, table_stride=1, lengths=at, out=at, requests=1,
+                  heads=1, kv_heads=1, dim=64, columns=1, pages=1, page_size=16)
+    for name in ("block_table", "lengths"):
+        assert lib.dlrb200_paged_attention(ref(_lib.PagedAttentionArgs(**{**attend, name: at + 2})), None) == 3, name
