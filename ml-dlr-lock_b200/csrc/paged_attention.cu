@@ -2,8 +2,8 @@
 //
 //   o_h = sum_j softmax_j(scale * q_h . k_j) v_j     over the tokens j of the request; zeros where there are none
 //
-// Bound by memory: the keys and values of a request are read once for all query heads that share them, and each value read serves
-// one multiply-add for each of these heads, far below what the tensor cores give.
+// Bound by memory: the keys and values of a request are read once for up to 16 query heads that share them (more: once for each 16),
+// and each value read serves one multiply-add for each of these heads, far below what the tensor cores give.
 //
 // Split.  The work is a list of tiles of 64 tokens: request by request, key-value head by key-value head.  It is cut into
 // equal runs, a few for each CTA, wherever the cuts fall: short requests share a CTA, a long one is spread over all of them, ragged
@@ -17,7 +17,7 @@
 // output of its tokens in registers; the warps of a CTA are joined at the end of a segment.  Scores are (heads x tokens), the
 // output is turned round, (values x heads): the scores' registers then are the second product's operand as they are, and the
 // output of eight heads takes half the registers that 16 rows would.  A softmax weight enters that product as a sum of 16-bit terms,
-// three in bf16 (all 24 bits of it), two in fp16 (22 bits).
+// three in bf16 (all 24 bits of it; two, 16 bits, where more than eight heads share keys), two in fp16 (22 bits).
 #include "paged_attention.h"
 
 #include <cuda_bf16.h>
@@ -38,19 +38,22 @@ constexpr int kUnit = 16;                        // tokens of a warp's step
 constexpr int kTile = kUnit * kWarpsA;           // tokens of a tile
 // CTAs of an SM for heads of `dim`, nt groups of eight sharing keys: as many as registers and shared memory allow.  More warps
 // count for more than more copies in flight: a warp's step is a chain of dependent instructions (460 MB, us: 6 heads of 128 with
-// 3 CTAs of 3 or 4 halves 77, 2 CTAs of 5 or 6 halves 80; 3 heads of 256 with 2 CTAs of 2 halves 76, of 3 halves 80, one CTA of 4 85).
+// 3 CTAs of 3 halves 80, of 4 halves 81, 2 CTAs of 5 or 6 halves 82; 3 heads of 256 with 2 CTAs of 2 halves 82, of 3 halves 93, one CTA
+// of 4 86).
 constexpr int ctas_per_sm(int dim, int nt) { return dim == 64 ? 4 : dim == 96 ? (nt == 1 ? 4 : 3) : dim == 128 ? 3 : 2; }
 constexpr int kMostCtasPerSm = 4;
 // Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (kernel and
-// join, us): 64 ragged requests of up to 8000 tokens, 8 heads of 128: 173 / 168 / 164 / 164; one of 131072: 93 / 92 / 92 / 94; 200
-// of up to 1500, 12 heads of 64: 83 / 84 / 83 / 90 with at least 32 / 8 / 32 / 8 tiles.
+// join, us): 64 ragged requests of up to 8000 tokens, 8 heads of 128: 173 / 171 / 167 / 166; one of 131072: 93 / 93 / 93 / 93; 200
+// of up to 1500, 12 heads of 64: 92 / 94 / 94 / 94 with at least 32 tiles, 84 with 8 (84 and 83 when 32 was chosen, before the output was
+// turned round); heads of 128 with at least 8: as with 16.
 constexpr int kWaves = 4;
 constexpr int least_run(int dim) { return dim == 64 ? 32 : 16; }
 constexpr int kMostShares = 8;                   // CTAs of a cluster
 // Tiles of a share up to which a cluster for each segment is taken instead of the runs and their join, by what the table could
-// hold (the host knows no lengths).  us, runs / clusters, contexts of one length, then ragged ones: 1 request of 513 tokens, 8
-// heads of 128, 2 tiles: 5.7 / 4.7; 8 of 768, 2 tiles: 9.7 / 7.1, 8.7 / 6.8; 8 of 2000, 8 tiles: 15.6 / 11.7, 12.5 / 10.5; 32 of
-// 768, 12 tiles: 20.9 / 16.2, 15.0 / 13.4; 256 of 700, 11 tiles: 135 / 119, 69 / 63.  Above: 64 of 1000, 16 tiles: 51 / 57, 34 / 31.
+// hold (the host knows no lengths).  us, runs / clusters, contexts of one length, then ragged ones, 8 heads of 128, up to 40 caches
+// in turn (400 MB, above what L2 holds, but for the first case): 1 request of 513 tokens, 2 tiles: 7.1 / 5.3; 8 of 768, 2 tiles: 11.2 /
+// 7.9, 10.1 / 6.8; 8 of 2000, 8 tiles: 19.2 / 13.7, 14.4 / 11.3; 32 of 768, 12 tiles: 31.9 / 18.4, 24.0 / 14.8; 256 of 700, 11 tiles:
+// 123 / 115, 73 / 63.  Above: 64 of 1000, 16 tiles: 48 / 56, 29 / 28.
 constexpr int kShort = 12;
 constexpr int kMostSms = 160;
 constexpr int kMostParts = kMostCtasPerSm * kMostSms * kWaves;
@@ -60,8 +63,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // right to 2^-16 of itself down to 2^-24 of the largest one, to 2^-40 of the largest one down to 2^-39 of it, and to 2^-38 below.
 template <typename T>
 constexpr float kWeightUp = __is_same(T, __half) ? 32768.f : 1.f;
-template <typename T>
-constexpr int kTerms = __is_same(T, __half) ? 2 : 3;
+// Terms of a weight: those of fp16, and of bf16 for NT groups of eight heads that share keys.
+template <typename T, int NT>
+constexpr int kTerms = __is_same(T, __half) || NT > 1 ? 2 : 3;
 template <typename T>
 constexpr float kLeastTerm = __is_same(T, __half) ? 0x1p-24f : 0x1p-126f;
 
@@ -139,11 +143,13 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 
 // Two weights as sums of 16-bit terms.  All terms of a weight above 0 are above 0: a term that is zero or negative would turn an
 // infinite value into NaN or the other infinity, by the weight's bits.  Hence the rounding toward zero; the last term takes what is left.
-// (Two terms of bf16 leave outputs 1e-4 away from those of fp32 weights, three 5e-5, which is what sums in another order do.  64
-// ragged requests of up to 8000 tokens: 164.4 us with two terms, 165.1 with three; one of 131072: 91.8 and 93.0; 64 of up to 4000, 16
-// heads of 64 to a key head: 65.8 and 73.1.  Two signed terms, and the tokens once more where an output is not finite: 166.3, 93.0, 69.3.)
-template <typename T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t (&term)[kTerms<T>]) {
+// (Outputs are 1e-4 away from those of fp32 weights with two terms of bf16, 5e-5 with three, which is what sums in another order
+// do; both far below their rounding to bf16.  us with two signed terms / three: 64 ragged requests of up to 8000 tokens, 4 heads of
+// 128 to a key head 164.4 / 165.1; one of 131072, 8 heads to a key head 91.8 / 93.0.  460 MB of ragged requests, 12 heads to a key
+// head, two signed terms / two / three: heads of 64 130 / 131 / 145, of 128 90 / 90 / 96, of 256 135 / 135 / 146.  Two signed terms,
+// and the tokens once more where an output is not finite, in these five cases: 166.3, 93.0, 139, 91.5, 137.)
+template <typename T, int TERMS>
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&term)[TERMS]) {
     const float least_x = x > 0.f ? kLeastTerm<T> : 0.f, least_y = y > 0.f ? kLeastTerm<T> : 0.f;
     if constexpr (__is_same(T, __half)) {      // (half of the least term less: together the two are off by as much up as down)
         term[0] = toward_zero2<T>(fmaxf(x - kLeastTerm<T> / 2, least_x), fmaxf(y - kLeastTerm<T> / 2, least_y));
@@ -151,11 +157,11 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&term)[kTerms
         term[0] = toward_zero2<T>(x, y);
     }
 #pragma unroll
-    for (int i = 1; i < kTerms<T>; ++i) {
+    for (int i = 1; i < TERMS; ++i) {
         const float2 before = floats2<T>(term[i - 1]);
         x = fmaxf(x - before.x, least_x);
         y = fmaxf(y - before.y, least_y);
-        term[i] = i + 1 < kTerms<T> ? toward_zero2<T>(x, y) : pack2<T>(x, y);
+        term[i] = i + 1 < TERMS ? toward_zero2<T>(x, y) : pack2<T>(x, y);
     }
 }
 
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
             }
             const int valid = tokens - (first + step * kWarpsA) * kUnit;
             float alpha[NT];
-            uint32_t weight[NT][2][kTerms<T>];
+            uint32_t weight[NT][2][kTerms<T, NT>];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float x[4];
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(kThreadsA, Shape<D, NT>::kCtasPerSm) paged_att
                 uint32_t a0, a1, a2, a3;
                 ldmatrix_x4_trans(v_at + t * 32, a0, a1, a2, a3);
 #pragma unroll
-                for (int i = 0; i < kTerms<T>; ++i)
+                for (int i = 0; i < kTerms<T, NT>; ++i)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma16816<T>(o[n][t], a0, a1, a2, a3, weight[n][0][i], weight[n][1][i]);
             }
