@@ -316,7 +316,25 @@ class RotaryTables:
     def __init__(self, model, positions: Optional[int] = None):
         self._rotary = model.model.rotary_emb
         self._positions = int(positions if positions is not None else model.config.max_position_embeddings)
-        self._made = {}
+        self._made, self._frequencies = {}, None
+
+    @classmethod
+    def of(cls, model) -> "RotaryTables":
+        """A model's tables, kept with its rotary embedding: a graph that was captured with them reads them after the modules were
+        switched back or fused again.  Where the frequencies have changed since, new ones beside them."""
+        rotary = model.model.rotary_emb
+        kept, new = rotary.__dict__.setdefault("_dlr_tables", []), cls(model)
+        for tables in kept:
+            if tables._positions == new._positions and tables._are_of(rotary):
+                return tables
+        kept.append(new)
+        return new
+
+    def _are_of(self, rotary) -> bool:
+        if self._frequencies is None:            # (none made yet)
+            return self._rotary is rotary
+        scale, frequencies = self._frequencies
+        return scale == float(getattr(rotary, "attention_scaling", 1.0)) and torch.equal(frequencies, rotary.inv_freq.detach().cpu())
 
     @staticmethod
     def fixed(model) -> bool:
@@ -335,6 +353,8 @@ class RotaryTables:
             if torch.cuda.is_current_stream_capturing():
                 return made                      # (a graph's hold nothing before its first replay: they stay its own)
             torch.cuda.current_stream(device).synchronize()
+        if self._frequencies is None:
+            self._frequencies = (scale, self._rotary.inv_freq.detach().cpu().clone())
         self._made[device] = made
         return made
 
@@ -406,7 +426,7 @@ def fuse_decoder_layers(model, enabled: bool = True, attention: bool = False) ->
     Returns how many layers were switched."""
     import types
     n = 0
-    tables = RotaryTables(model) if enabled and attention and RotaryTables.fixed(model) else None
+    tables = RotaryTables.of(model) if enabled and attention and RotaryTables.fixed(model) else None
     for layer in model.model.layers:
         if not _fusable(layer):
             continue

@@ -63,3 +63,44 @@ def test_tables_made_on_one_stream_are_there_for_another():
         second.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         first.synchronize()
+
+
+def test_a_captured_graph_outlives_the_switch_of_its_modules():
+    import copy
+    import dlr_lock_b200 as D
+    model = _model(layers=2)
+    ids = torch.randint(0, 1000, (2, 16), device=DEV)
+    with torch.no_grad():
+        D.fuse_decoder_layers(model, True, attention=True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = model(ids).logits
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = model(ids).logits
+        tables = model.model.layers[0].self_attn._rotary_tables
+        D.fuse_decoder_layers(model, True)
+        D.fuse_decoder_layers(model, True, attention=True)
+        assert model.model.layers[0].self_attn._rotary_tables is tables
+        D.fuse_decoder_layers(model, True)
+        del tables
+        others = [torch.full((1 << 14,), float("nan"), device=DEV) for _ in range(64)]
+        graph.replay()
+        assert torch.equal(out, want) and all(torch.isnan(t).all() for t in others)
+        # a copy has tables of its own, and so have other frequencies
+        D.fuse_decoder_layers(model, True, attention=True)
+        twin = copy.deepcopy(model)
+        assert twin.model.layers[0].self_attn._rotary_tables is not model.model.layers[0].self_attn._rotary_tables
+        assert torch.equal(twin(ids).logits, want)
+        twin.model.rotary_emb.inv_freq.mul_(0.5)
+        D.fuse_decoder_layers(twin, True, attention=True)
+        other = twin(ids).logits
+        fresh = copy.deepcopy(model)
+        del fresh.model.rotary_emb.__dict__["_dlr_tables"]
+        fresh.model.rotary_emb.inv_freq.mul_(0.5)
+        D.fuse_decoder_layers(fresh, True, attention=True)
+        assert torch.equal(other, fresh(ids).logits) and not torch.equal(other, want)
+        graph.replay()
+        assert torch.equal(out, want)
