@@ -306,7 +306,9 @@ DLRB200_API int dlrb200_qk_norm_rope_backward(const dlrb200_norm_rope_grad_args*
  * the keys and values of head h / (heads / kv_heads) of request r's pages; zeros
  * where lengths[r] is 0.  Lengths are read on the device (held to 0 .. columns
  * pages), so that a captured call follows them.  A table entry outside the cache
- * is never followed: it counts as a page of zeros.  dim is 64, 96, 128 or 256,
+ * is never followed: it counts as a page of zeros.  An infinite value among a
+ * request's tokens comes out infinite (infinities of both signs, and NaN, as
+ * NaN) unless its weight is 0 in fp32.  dim is 64, 96, 128 or 256,
  * pages have at least 16 tokens.  workspace: 16-byte aligned, used only during
  * the call; calls that overlap need one each. */
 typedef struct dlrb200_paged_attention_args {

@@ -11,7 +11,8 @@ A cache is a pair of (pages, kv_heads, page tokens, dim) tensors, bf16 or fp16, 
 attention and cache, has no counterpart of these.
 
 Every call is asynchronous on the current stream of the tensors' device, never synchronises, and can be captured in a CUDA
-graph; workspaces are taken from torch's allocator per call, so that captured graphs share none.
+graph; workspaces are taken from torch's allocator per call, so that captured graphs share none.  Forward-mode tangents are
+refused.
 """
 from __future__ import annotations
 
@@ -317,7 +318,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table`` (requests, columns) and ``lengths`` int32.  ``heads`` is a multiple of the caches' heads, each of which
     serves that many neighbouring query heads; dim is 64, 96, 128 or 256.  ``scale`` is 1 / sqrt(dim) unless given.  Lengths
     are read on the device: a captured call follows them.  A table entry outside the caches counts as a page of zeros and
-    is never followed.  Scores, softmax and sums are fp32.  No gradient.
+    is never followed.  Scores, softmax and sums are fp32; the weights enter their product with the values to 16 bits at least
+    (fp16: down to 2^-24 of the largest).  An infinite value of a request's token comes out infinite.  No gradient.
     """
     out = _native().paged_attention(q, k_cache, v_cache, block_table, lengths, scale)
     if out is not None and type(out) is not int:
