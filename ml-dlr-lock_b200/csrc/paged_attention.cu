@@ -44,8 +44,8 @@ constexpr int ctas_per_sm(int dim, int nt) { return dim == 64 ? 4 : dim == 96 ? 
 constexpr int kMostCtasPerSm = 4;
 // Runs for each resident CTA, and tiles of a run below which there is one for each.  Measured with 1 / 2 / 4 / 6 runs (kernel and
 // join, us): 64 ragged requests of up to 8000 tokens, 8 heads of 128: 173 / 171 / 167 / 166; one of 131072: 93 / 93 / 93 / 93; 200
-// of up to 1500, 12 heads of 64: 92 / 94 / 94 / 94 with at least 32 tiles, 84 with 8 (32 was chosen before the output was turned round, when it took
-// 83); heads of 128 with at least 8: as with 16.
+// of up to 1500, 12 heads of 64: 92 / 94 / 94 / 94 with at least 32 tiles, 84 with 8 (32 was chosen before the output was turned
+// round, when it took 83); heads of 128 with at least 8: as with 16.
 constexpr int kWaves = 4;
 constexpr int least_run(int dim) { return dim == 64 ? 32 : 16; }
 constexpr int kMostShares = 8;                   // CTAs of a cluster
